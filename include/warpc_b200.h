@@ -210,6 +210,59 @@ int wg_noalloc_max_flags(void);
 int wg_kernel_count(void);
 const char* wg_kernel_name(int kernel_id);
 
+/* ------------------------------------------------------------------ 8-bit operators
+ * The product of 8-bit integers with a scale for each token and each channel, and what makes its operands (no counterpart
+ * in the reference).  Together they are a projection of a language model in 8 bits: a row of activations (a token) goes
+ * through wg_norm_quantise_rows or wg_quantise_rows, a weight matrix once through wg_quantise_rows (a row is a channel),
+ * and wg_int8_launch multiplies what they wrote.
+ *
+ * Value types: WG_BF16, WG_FP16, WG_FP32.  Rows are `ld*` elements apart (>= the row's length); every ld is 64 bits.  No entry
+ * synchronises or allocates but wg_int8_plan_create / _destroy / _last_device_status, so all of them may be captured into a
+ * graph; calls on different streams share nothing but a plan's status words, which only a wait that gives up writes. */
+enum { WG_BF16 = 0, WG_FP16 = 1, WG_FP32 = 2 };
+
+/* q[m, k] = 127 x[m, k] / a rounded half to even, dScale[m] = a / 127 with a = max_k |x[m, k]|: exactly, in every type.
+ * A row of zeros gives q = 0 and scale 0; a row that holds an infinity or a NaN gives q = 0 and scale NaN (so its product
+ * is NaN).  Columns K..ldq of dQ are left as they were.  Any alignment and stride works; 16-byte aligned rows of x and 8-byte
+ * aligned rows of q are the fast ones.  M = 0 is no work. */
+int wg_quantise_rows(int device, int M, int K, int dtype, const void* dX, long long ldx, signed char* dQ, long long ldq, float* dScale,
+                     void* cuda_stream);
+/* The root-mean-square norm with the residual's addition, to 8 bits: h = x + r rounded to the rows' type and written to dH
+ * (dR and dH both NULL: h = x), t = h * w in 32 bits, dScale[m] = max_k |t| / 127 / sqrt(mean_k(h^2) + eps) and
+ * q = 127 t / max_k |t| rounded half to even -- the norm of h times w, in 8 bits.  dW has K values of the rows' type.  dH may be
+ * dX or dR itself (same stride); otherwise the outputs overlap nothing.  Zeros and values that are not finite (t not
+ * finite in 32 bits among them) as in wg_quantise_rows. */
+int wg_norm_quantise_rows(int device, int M, int K, int dtype, const void* dX, long long ldx, const void* dR, long long ldr, const void* dW, float eps,
+                          void* dH, long long ldh, signed char* dQ, long long ldq, float* dScale, void* cuda_stream);
+
+/* The program of a product: WG_INT8_GEMV (tile_m >= M in {1, 2, 4, 8}; `split` warps share a channel's K), WG_INT8_FEW (tile_m
+ * in {32, 64, 128} tokens x 128 channels a CTA, `split` <= 8 CTAs of a cluster share K), WG_INT8_TILE (tile_m x tile_n =
+ * 256 x 256 or 256 x 128 on a CTA pair, 128 x 128 or 128 x 64 on a CTA; split 1). */
+enum { WG_INT8_GEMV = 1, WG_INT8_FEW = 2, WG_INT8_TILE = 3 };
+typedef struct wg_int8_info {
+  int kernel, tile_m, tile_n, split;                        /* what names a program */
+  int tiles, grid, cluster, threads, dynsmem, depth;        /* its launch */
+} wg_int8_info;
+int wg_int8_choose(int M, int N, int K, wg_int8_info* out);
+
+/* A plan for one weight matrix: dBt is N x K signed 8-bit (a row a channel), 16-byte aligned, ldb a multiple of 16; dScaleB
+ * N floats and dBias N floats (or NULL), 16-byte aligned; the output is out_dtype.  K <= 131071 (WG_E_LIMIT beyond: the 32-bit sum
+ * cannot wrap below that).  The plan keeps the pointers, not copies. */
+int wg_int8_plan_create(int device, int N, int K, const signed char* dBt, long long ldb, const float* dScaleB, const float* dBias, int out_dtype, void** plan);
+/* C[m, n] = dScaleA[m] * dScaleB[n] * sum_k A[m, k] * Bt[n, k] (+ dBias[n]) for M tokens, on `cuda_stream`: the sum in 32-bit
+ * integers (exact; the same bits every launch, whatever the program), scaled in fp32, rounded once to the output type.  dA is M x K signed
+ * 8-bit, 16-byte aligned, lda a multiple of 16; ldc >= N, any alignment of dC (16-byte aligned rows are the fast ones).
+ * A row's last 16-byte piece is read whole; what it holds past K does not matter.  M = 0 is no work.  Launches of one plan on
+ * several streams at once are fine. */
+int wg_int8_launch(void* plan, int M, const signed char* dA, long long lda, const float* dScaleA, void* dC, long long ldc, void* cuda_stream);
+/* Name the program of the launches that follow (kernel, tile_m, tile_n, split; the rest is derived), NULL: the rule's again.
+ * WG_E_VARIANT where there is no such program; a launch with more tokens than a named gemv takes returns it too. */
+int wg_int8_plan_set_program(void* plan, const wg_int8_info* program);
+/* Bounded waits and their status, as wg_plan_set_timeout_ms and wg_last_device_status. */
+int wg_int8_plan_set_timeout_ms(void* plan, unsigned ms);
+int wg_int8_last_device_status(void* plan, unsigned out[4]);
+int wg_int8_plan_destroy(void* plan);
+
 const char* wg_strerror(int code);
 
 #ifdef __cplusplus

@@ -6,6 +6,7 @@ through ctypes.  There is no CPU fallback: without the shared library every entr
 """
 from .programs import Variant, LaunchInfo, choose, swapped, pair, one, realise, header, kernel_is_simple  # noqa: F401
 from .plan import Plan, HostPlan, DeviceWaitError  # noqa: F401
+from .int8 import Int8Info, Int8Plan, int8_choose, norm_quantise_rows, quantise_rows  # noqa: F401
 
 __all__ = ["Variant", "LaunchInfo", "choose", "swapped", "pair", "one", "realise", "header", "Plan", "HostPlan",
-           "DeviceWaitError"]
+           "DeviceWaitError", "Int8Info", "Int8Plan", "int8_choose", "norm_quantise_rows", "quantise_rows"]

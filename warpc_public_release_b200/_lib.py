@@ -9,6 +9,8 @@ WG_OK = 0
 WG_E_SHAPE, WG_E_VARIANT, WG_E_ARG, WG_E_NOKERNEL, WG_E_DEVICE_WAIT, WG_E_NODRIVER, WG_E_LIMIT = -1, -2, -3, -4, -5, -6, -7
 PROG_SWAPPED, PROG_PAIR, PROG_ONE = 0, 1, 2
 SM_100A, SM_103A = 100, 103
+TYPES = {"bf16": 0, "fp16": 1, "fp32": 2}
+INT8_GEMV, INT8_FEW, INT8_TILE = 1, 2, 3
 
 
 class Variant(ctypes.Structure):
@@ -37,6 +39,14 @@ class LaunchInfo(ctypes.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class Int8Info(ctypes.Structure):
+    """wg_int8_info: a program of the 8-bit product and its launch."""
+    _fields_ = [(n, ctypes.c_int) for n in ("kernel", "tile_m", "tile_n", "split", "tiles", "grid", "cluster", "threads", "dynsmem", "depth")]
+
+    def as_dict(self):
+        return {n: getattr(self, n) for n, _ in self._fields_}
+
+
 _lib = None
 
 
@@ -49,7 +59,7 @@ def lib():
         raise RuntimeError("libwarpc_b200.so is not built (run `python -c 'import __graft_entry__ as g; g.build()'` "
                            "or `make -C warpc_public_release_b200/csrc`); there is no CPU fallback")
     l = ctypes.CDLL(LIB_PATH)
-    vp, i, u = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint
+    vp, i, u, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint, ctypes.c_longlong
     PV, PL = ctypes.POINTER(Variant), ctypes.POINTER(LaunchInfo)
     sig = {
         "wg_choose": ([i, i, i, i, PV], i),
@@ -81,6 +91,15 @@ def lib():
         "wg_launch_noalloc": ([i, PV, i, i, i, vp, vp, vp, vp], i),
         "wg_noalloc_status": ([i, ctypes.POINTER(u * 4)], i),
         "wg_noalloc_max_flags": ([], i),
+        "wg_quantise_rows": ([i, i, i, i, vp, ll, vp, ll, vp, vp], i),
+        "wg_norm_quantise_rows": ([i, i, i, i, vp, ll, vp, ll, vp, ctypes.c_float, vp, ll, vp, ll, vp, vp], i),
+        "wg_int8_choose": ([i, i, i, ctypes.POINTER(Int8Info)], i),
+        "wg_int8_plan_create": ([i, i, i, vp, ll, vp, vp, i, ctypes.POINTER(vp)], i),
+        "wg_int8_plan_set_program": ([vp, ctypes.POINTER(Int8Info)], i),
+        "wg_int8_plan_set_timeout_ms": ([vp, u], i),
+        "wg_int8_launch": ([vp, i, vp, ll, vp, vp, ll, vp], i),
+        "wg_int8_last_device_status": ([vp, ctypes.POINTER(u * 4)], i),
+        "wg_int8_plan_destroy": ([vp], i),
         "wg_kernel_count": ([], i),
         "wg_kernel_name": ([i], ctypes.c_char_p),
         "wg_strerror": ([i], ctypes.c_char_p),

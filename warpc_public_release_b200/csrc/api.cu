@@ -14,6 +14,7 @@
 
 #include "../../include/warpc_b200.h"
 #include "gemm_kernel.cuh"
+#include "host_cuda.h"
 #include "kernel_table.h"
 
 namespace {
@@ -66,23 +67,6 @@ const wb_kernel_entry* table() {
   return t;
 }
 constexpr int kKernels = 19;
-
-// ------------------------------------------------------------------ driver entry points
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
 
 // A row-major rows x cols matrix, box = box_rows x box_cols, 128-byte swizzle (operands) or none
 // (the C staging boxes), zero fill
@@ -143,35 +127,6 @@ struct Plan {
   std::vector<cudaEvent_t> ev_a, ev_b, ev_mm;  // launches carry the programmatic stream serialization attribute
   int M = 0, N = 0, K = 0;
 };
-
-#define WG_CUDA(call)                          \
-  do {                                         \
-    cudaError_t e_ = (call);                   \
-    if (e_ != cudaSuccess) return int(e_);     \
-  } while (0)
-
-// Makes `device` current for the length of an entry point and gives the caller's device back on
-// the way out, so one host thread can drive plans on several GPUs in turn.
-struct DeviceGuard {
-  int prev = -1;
-  bool changed = false;
-  cudaError_t err = cudaSuccess;
-  explicit DeviceGuard(int device) {
-    err = cudaGetDevice(&prev);
-    if (err == cudaSuccess && prev != device) {
-      err = cudaSetDevice(device);
-      changed = err == cudaSuccess;
-    }
-  }
-  ~DeviceGuard() {
-    if (changed) cudaSetDevice(prev);
-  }
-  DeviceGuard(const DeviceGuard&) = delete;
-  DeviceGuard& operator=(const DeviceGuard&) = delete;
-};
-#define WG_ON_DEVICE(device)        \
-  DeviceGuard guard_(device);       \
-  if (guard_.err != cudaSuccess) return int(guard_.err)
 
 void launch_config(const wg_launch_info& li, cudaStream_t stream, bool dependent, cudaLaunchConfig_t* cfg, cudaLaunchAttribute attr[2]) {
   std::memset(cfg, 0, sizeof *cfg);

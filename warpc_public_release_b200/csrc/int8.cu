@@ -1,0 +1,356 @@
+// C ABI of the 8-bit operators: rows to 8 bits (with or without the root-mean-square norm before it), and the product of
+// 8-bit integers with a scale for each token and channel.
+#include <algorithm>
+#include <cstring>
+#include <new>
+
+#include "../../include/warpc_b200.h"
+#include "host_cuda.h"
+#include "int8_kernel.cuh"
+#include "rows_kernel.cuh"
+
+namespace {
+
+using namespace wb;
+
+constexpr int kSms = 148;
+
+bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+bool known_type(int dtype) { return dtype == WG_BF16 || dtype == WG_FP16 || dtype == WG_FP32; }
+int type_size(int dtype) { return dtype == WG_FP32 ? 4 : 2; }
+
+// ------------------------------------------------------------------ rows
+struct RowLaunch {
+  int vpt, threads, rows, grid;
+  bool loop;
+};
+
+// How a row is spread: `slots` vectors of 16 bytes.  A warp a row up to 64 vectors (no barrier); else a block a row, two
+// vectors a thread while a block holds the row so (the next row's loads fit in registers beside them), one where there
+// are too few rows to fill the machine and only a row's own latency counts.
+RowLaunch row_launch(int M, int slots) {
+  RowLaunch l;
+  l.loop = false;
+  if (slots <= 64) {
+    l.vpt = slots <= 32 ? 1 : 2, l.threads = 32, l.rows = M > 4 * kSms ? 8 : 1;
+  } else {
+    l.rows = 1;
+    l.vpt = slots <= 1024 && M <= 2 * kSms ? 1 : slots <= 2048 ? 2 : 8;
+    if (slots > 4096) l.vpt = 4, l.loop = true;
+    l.threads = l.loop ? 512 : std::min(1024, (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32);
+  }
+  const int per_sm = std::max(1, 1024 / (l.threads * l.rows));
+  l.grid = std::min((M + l.rows - 1) / l.rows, kSms * per_sm);
+  return l;
+}
+
+template <class T, bool NORM, bool RES, bool VEC>
+int launch_rows(const RowParams& p, cudaStream_t stream) {
+  const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E);
+  const dim3 block(unsigned(l.threads), unsigned(l.rows)), grid(unsigned(l.grid));
+  if (l.loop) rows_kernel<T, NORM, RES, VEC, 4, true><<<grid, block, 0, stream>>>(p);
+  else if (l.vpt == 1) rows_kernel<T, NORM, RES, VEC, 1, false><<<grid, block, 0, stream>>>(p);
+  else if (l.vpt == 2) rows_kernel<T, NORM, RES, VEC, 2, false><<<grid, block, 0, stream>>>(p);
+  else rows_kernel<T, NORM, RES, VEC, 8, false><<<grid, block, 0, stream>>>(p);
+  return int(cudaGetLastError());
+}
+
+template <class T, bool NORM, bool RES>
+int launch_rows_as(const RowParams& p, cudaStream_t stream) {
+  const unsigned bytes = 16, qbytes = RowVec<T>::E;
+  auto whole = [&](long long ld, unsigned size) { return p.M == 1 || (ld * size) % bytes == 0; };
+  bool vec = aligned(p.x, bytes) && whole(p.ldx, sizeof(T)) && aligned(p.q, qbytes) && (p.M == 1 || p.ldq % qbytes == 0);
+  if (NORM) vec = vec && aligned(p.w, bytes);
+  if (RES) vec = vec && aligned(p.r, bytes) && aligned(p.h, bytes) && whole(p.ldr, sizeof(T)) && whole(p.ldh, sizeof(T));
+  return vec ? launch_rows<T, NORM, RES, true>(p, stream) : launch_rows<T, NORM, RES, false>(p, stream);
+}
+
+template <bool NORM, bool RES>
+int launch_rows_of(int dtype, const RowParams& p, cudaStream_t stream) {
+  switch (dtype) {
+    case WG_BF16: return launch_rows_as<__nv_bfloat16, NORM, RES>(p, stream);
+    case WG_FP16: return launch_rows_as<__half, NORM, RES>(p, stream);
+    default: return launch_rows_as<float, NORM, RES>(p, stream);
+  }
+}
+
+// ------------------------------------------------------------------ the product
+struct I8Plan {
+  int device = 0, N = 0, K = 0, out = 0;
+  const int8_t* Bt = nullptr;
+  long long ldb = 0;
+  const float *sb = nullptr, *bias = nullptr;
+  CUtensorMap map_b128, map_b64;  // the weights in boxes of 128 and of 64 rows
+  uint32_t* d_status = nullptr;
+  unsigned long long timeout_ns = 2000ull * 1000ull * 1000ull;
+  wg_int8_info named{};  // the program a caller named, or kernel 0
+};
+
+int encode_rows(CUtensorMap* map, CUtensorMapDataType type, int size, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return WG_E_NODRIVER;
+  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(ld) * cuuint64_t(size)};
+  cuuint32_t box[2] = {cuuint32_t(128 / size), cuuint32_t(box_rows)}, estr[2] = {1, 1};
+  const CUresult r = enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? WG_OK : int(r);
+}
+
+constexpr size_t kI8MaxSmem = 232448;
+constexpr int kI8MaxDepth = 16;
+
+// ring stages that fit beside `fixed` bytes
+int ring_depth(size_t fixed, size_t stage, int most) { return int(std::min<size_t>(size_t(most), (kI8MaxSmem - fixed) / stage)); }
+
+// The launch of a named program; WG_E_VARIANT where there is none.
+int i8_derive(int M, int N, int K, wg_int8_info* o) {
+  const int kt = (K + 127) / 128;
+  auto up = [](int a, int b) { return int(((long long)a + b - 1) / b); };
+  o->threads = 256, o->depth = 0, o->dynsmem = 0, o->cluster = 1;
+  if (o->kernel == WG_INT8_GEMV) {
+    if (o->tile_m != 1 && o->tile_m != 2 && o->tile_m != 4 && o->tile_m != 8) return WG_E_VARIANT;
+    if (M > o->tile_m) return WG_E_VARIANT;
+    if (o->split != 1 && o->split != 2 && o->split != 4 && o->split != 8) return WG_E_VARIANT;
+    o->tile_n = 4 * (8 / o->split), o->tiles = up(N, o->tile_n), o->grid = o->tiles;
+    return WG_OK;
+  }
+  if (o->kernel == WG_INT8_FEW) {
+    if ((o->tile_m != 32 && o->tile_m != 64 && o->tile_m != 128) || o->tile_n != 128) return WG_E_VARIANT;
+    if (o->split < 1 || o->split > 8 || o->split > kt) return WG_E_VARIANT;
+    const size_t stage = size_t(128 + o->tile_m) * 128, fixed = 1024 + sizeof(I8Ctrl) + size_t(o->split) * up(o->tile_m, o->split) * 512;
+    o->depth = ring_depth(fixed, stage, std::min(12, std::max(2, up(kt, o->split))));
+    o->dynsmem = int(fixed + o->depth * stage), o->cluster = o->split;
+    const long long tiles = (long long)up(M, o->tile_m) * up(N, 128);
+    if (tiles * o->split > 0x7fffffffll) return WG_E_LIMIT;
+    o->tiles = int(tiles), o->grid = o->tiles * o->split;
+    return WG_OK;
+  }
+  if (o->kernel == WG_INT8_TILE) {
+    const int cg = o->tile_m / 128;
+    const bool known = (o->tile_m == 256 && (o->tile_n == 256 || o->tile_n == 128)) || (o->tile_m == 128 && (o->tile_n == 128 || o->tile_n == 64));
+    if (!known || o->split != 1) return WG_E_VARIANT;
+    const size_t stage = size_t(128 + o->tile_n / cg) * 128, fixed = 1024 + sizeof(I8Ctrl) + 4 * 2 * 4096;
+    o->depth = ring_depth(fixed, stage, 8);
+    o->dynsmem = int(fixed + o->depth * stage), o->cluster = cg;
+    const long long tiles = (long long)up(M, o->tile_m) * up(N, o->tile_n);
+    if (tiles > 0x3fffffffll) return WG_E_LIMIT;
+    o->tiles = int(tiles), o->grid = cg * std::min(o->tiles, kSms / cg);
+    return WG_OK;
+  }
+  return WG_E_VARIANT;
+}
+
+int i8_choose(int M, int N, int K, wg_int8_info* o) {
+  std::memset(o, 0, sizeof *o);
+  const int kt = (K + 127) / 128;
+  auto up = [](int a, int b) { return (a + b - 1) / b; };
+  if (M <= 4) {
+    o->kernel = WG_INT8_GEMV, o->tile_m = M <= 1 ? 1 : M <= 2 ? 2 : 4, o->split = 1;
+    while (o->split < 8 && up(N, 32 / o->split) < 2 * kSms && K > 1024 * o->split) o->split *= 2;
+  } else if (M <= 128) {
+    o->kernel = WG_INT8_FEW, o->tile_m = M <= 32 ? 32 : M <= 64 ? 64 : 128, o->tile_n = 128;
+    o->split = std::max(1, std::min(std::min(8, kt), kSms / up(N, 128)));
+  } else {
+    // cycles of a wave: k-steps at the slower of the tensor pipe and the loads, and what a tile's end costs
+    static const struct { int m, n, step, end; } tiles[] = {{256, 256, 512, 5000}, {256, 128, 340, 3500}, {128, 128, 440, 3500}, {128, 64, 330, 2500}};
+    double best = 0;
+    o->kernel = WG_INT8_TILE, o->split = 1;
+    for (const auto& t : tiles) {
+      const long long n = (long long)up(M, t.m) * up(N, t.n), slots = kSms / (t.m / 128), waves = (n + slots - 1) / slots;
+      const double cost = double(waves) * kt * t.step + t.end;
+      if (best == 0 || cost < best) best = cost, o->tile_m = t.m, o->tile_n = t.n;
+    }
+  }
+  return i8_derive(M, N, K, o);
+}
+
+template <class F>
+int launch(F* fn, const wg_int8_info& li, cudaStream_t stream, void** args) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = dim3(unsigned(li.grid)), cfg.blockDim = dim3(unsigned(li.threads));
+  cfg.dynamicSmemBytes = size_t(li.dynsmem), cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(li.cluster), attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = li.cluster > 1 || li.kernel == WG_INT8_FEW ? 1 : 0;
+  return int(cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(fn), args));
+}
+
+// The kernels of one output type; `set_up` raises their shared-memory limit instead of launching.
+template <int OUT>
+struct I8Kernels {
+  static int set_up() {
+    const void* fns[] = {(const void*)i8_tile_kernel<I8Cfg<2, 256>, OUT>, (const void*)i8_tile_kernel<I8Cfg<2, 128>, OUT>,
+                         (const void*)i8_tile_kernel<I8Cfg<1, 128>, OUT>, (const void*)i8_tile_kernel<I8Cfg<1, 64>, OUT>,
+                         (const void*)i8_few_kernel<I8Cfg<1, 32>, OUT>,   (const void*)i8_few_kernel<I8Cfg<1, 64>, OUT>,
+                         (const void*)i8_few_kernel<I8Cfg<1, 128>, OUT>};
+    for (const void* fn : fns) WG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kI8MaxSmem)));
+    return WG_OK;
+  }
+  static int run(const wg_int8_info& li, cudaStream_t stream, CUtensorMap* a, CUtensorMap* b, CUtensorMap* c, I8Params* p) {
+    if (li.kernel == WG_INT8_GEMV) {
+      void* args[] = {p};
+      switch (li.tile_m) {
+        case 1: return launch(&i8_gemv_kernel<1, 4, OUT>, li, stream, args);
+        case 2: return launch(&i8_gemv_kernel<2, 4, OUT>, li, stream, args);
+        case 4: return launch(&i8_gemv_kernel<4, 4, OUT>, li, stream, args);
+        default: return launch(&i8_gemv_kernel<8, 4, OUT>, li, stream, args);
+      }
+    }
+    if (li.kernel == WG_INT8_FEW) {
+      void* args[] = {a, b, p};
+      switch (li.tile_m) {
+        case 32: return launch(&i8_few_kernel<I8Cfg<1, 32>, OUT>, li, stream, args);
+        case 64: return launch(&i8_few_kernel<I8Cfg<1, 64>, OUT>, li, stream, args);
+        default: return launch(&i8_few_kernel<I8Cfg<1, 128>, OUT>, li, stream, args);
+      }
+    }
+    void* args[] = {a, b, c, p};
+    if (li.tile_m == 256) return li.tile_n == 256 ? launch(&i8_tile_kernel<I8Cfg<2, 256>, OUT>, li, stream, args) : launch(&i8_tile_kernel<I8Cfg<2, 128>, OUT>, li, stream, args);
+    return li.tile_n == 128 ? launch(&i8_tile_kernel<I8Cfg<1, 128>, OUT>, li, stream, args) : launch(&i8_tile_kernel<I8Cfg<1, 64>, OUT>, li, stream, args);
+  }
+};
+
+constexpr int kMaxK = 131071;  // 128 * 128 * K stays below 2^31
+
+}  // namespace
+
+extern "C" int wg_quantise_rows(int device, int M, int K, int dtype, const void* dX, long long ldx, signed char* dQ, long long ldq, float* dScale,
+                                void* cuda_stream) {
+  if (!known_type(dtype) || M < 0 || K <= 0 || ldx < K || ldq < K) return WG_E_ARG;
+  if (M == 0) return WG_OK;
+  if (!dX || !dQ || !dScale || !aligned(dX, unsigned(type_size(dtype))) || !aligned(dScale, 4)) return WG_E_ARG;
+  RowParams p;
+  std::memset(&p, 0, sizeof p);
+  p.x = dX, p.q = reinterpret_cast<int8_t*>(dQ), p.scale = dScale, p.ldx = ldx, p.ldq = ldq, p.M = M, p.K = K;
+  WG_ON_DEVICE(device);
+  return launch_rows_of<false, false>(dtype, p, static_cast<cudaStream_t>(cuda_stream));
+}
+
+extern "C" int wg_norm_quantise_rows(int device, int M, int K, int dtype, const void* dX, long long ldx, const void* dR, long long ldr, const void* dW,
+                                     float eps, void* dH, long long ldh, signed char* dQ, long long ldq, float* dScale, void* cuda_stream) {
+  if (!known_type(dtype) || M < 0 || K <= 0 || ldx < K || ldq < K || !(eps >= 0.0f)) return WG_E_ARG;
+  if ((dR == nullptr) != (dH == nullptr) || (dR && (ldr < K || ldh < K))) return WG_E_ARG;
+  if (M == 0) return WG_OK;
+  const unsigned size = unsigned(type_size(dtype));
+  if (!dX || !dW || !dQ || !dScale || !aligned(dX, size) || !aligned(dW, size) || !aligned(dR, size) || !aligned(dH, size) || !aligned(dScale, 4))
+    return WG_E_ARG;
+  if ((dH == dX && ldh != ldx) || (dH && dH == dR && ldh != ldr)) return WG_E_ARG;
+  RowParams p;
+  std::memset(&p, 0, sizeof p);
+  p.x = dX, p.r = dR, p.w = dW, p.h = dH, p.q = reinterpret_cast<int8_t*>(dQ), p.scale = dScale;
+  p.ldx = ldx, p.ldr = ldr, p.ldh = ldh, p.ldq = ldq, p.M = M, p.K = K, p.eps = eps;
+  WG_ON_DEVICE(device);
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  return dR ? launch_rows_of<true, true>(dtype, p, stream) : launch_rows_of<true, false>(dtype, p, stream);
+}
+
+extern "C" int wg_int8_choose(int M, int N, int K, wg_int8_info* out) {
+  if (!out || M <= 0 || N <= 0 || K <= 0) return WG_E_ARG;
+  if (K > kMaxK) return WG_E_LIMIT;
+  return i8_choose(M, N, K, out);
+}
+
+extern "C" int wg_int8_plan_create(int device, int N, int K, const signed char* dBt, long long ldb, const float* dScaleB, const float* dBias, int out_dtype,
+                                   void** plan) {
+  if (!plan) return WG_E_ARG;
+  *plan = nullptr;
+  if (!known_type(out_dtype) || N <= 0 || K <= 0 || ldb < K || ldb % 16 != 0) return WG_E_ARG;
+  if (!dBt || !dScaleB || !aligned(dBt, 16) || !aligned(dScaleB, 16) || !aligned(dBias, 16)) return WG_E_ARG;
+  if (K > kMaxK) return WG_E_LIMIT;
+  WG_ON_DEVICE(device);
+  I8Plan* pl = new (std::nothrow) I8Plan();
+  if (!pl) return WG_E_ARG;
+  pl->device = device, pl->N = N, pl->K = K, pl->out = out_dtype;
+  pl->Bt = reinterpret_cast<const int8_t*>(dBt), pl->ldb = ldb, pl->sb = dScaleB, pl->bias = dBias;
+  int r = encode_rows(&pl->map_b128, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dBt, N, K, ldb, 128);
+  if (r == WG_OK) r = encode_rows(&pl->map_b64, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dBt, N, K, ldb, 64);
+  if (r == WG_OK) r = int(cudaMalloc(&pl->d_status, 4 * sizeof(uint32_t)));
+  if (r == WG_OK) r = int(cudaMemsetAsync(pl->d_status, 0, 4 * sizeof(uint32_t), 0));
+  if (r == WG_OK) r = int(cudaStreamSynchronize(0));  // zero before any stream, blocking or not, can launch on the plan
+  if (r == WG_OK) r = out_dtype == WG_BF16 ? I8Kernels<I8_BF16>::set_up() : out_dtype == WG_FP16 ? I8Kernels<I8_FP16>::set_up() : I8Kernels<I8_FP32>::set_up();
+  if (r != WG_OK) {
+    wg_int8_plan_destroy(pl);
+    return r;
+  }
+  *plan = pl;
+  return WG_OK;
+}
+
+extern "C" int wg_int8_plan_set_program(void* plan, const wg_int8_info* program) {
+  I8Plan* pl = static_cast<I8Plan*>(plan);
+  if (!pl) return WG_E_ARG;
+  wg_int8_info named;
+  std::memset(&named, 0, sizeof named);
+  if (program) {
+    named.kernel = program->kernel, named.tile_m = program->tile_m, named.tile_n = program->tile_n, named.split = program->split;
+    wg_int8_info probe = named;
+    const int r = i8_derive(1, pl->N, pl->K, &probe);
+    if (r != WG_OK) return r;
+  }
+  pl->named = named;
+  return WG_OK;
+}
+
+extern "C" int wg_int8_plan_set_timeout_ms(void* plan, unsigned ms) {
+  I8Plan* pl = static_cast<I8Plan*>(plan);
+  if (!pl) return WG_E_ARG;
+  pl->timeout_ns = (ms ? ms : 2000u) * 1000000ull;
+  return WG_OK;
+}
+
+extern "C" int wg_int8_launch(void* plan, int M, const signed char* dA, long long lda, const float* dScaleA, void* dC, long long ldc, void* cuda_stream) {
+  I8Plan* pl = static_cast<I8Plan*>(plan);
+  if (!pl || M < 0) return WG_E_ARG;
+  const int size = type_size(pl->out);
+  if (lda < pl->K || lda % 16 != 0 || ldc < pl->N) return WG_E_ARG;
+  if (M == 0) return WG_OK;
+  if (!dA || !dScaleA || !dC || !aligned(dA, 16) || !aligned(dScaleA, 4) || !aligned(dC, unsigned(size))) return WG_E_ARG;
+  wg_int8_info li = pl->named;
+  int r = li.kernel ? i8_derive(M, pl->N, pl->K, &li) : i8_choose(M, pl->N, pl->K, &li);
+  if (r != WG_OK) return r;
+  I8Params p;
+  std::memset(&p, 0, sizeof p);
+  p.M = M, p.N = pl->N, p.K = pl->K, p.kt = (pl->K + 127) / 128;
+  p.tiles_m = int(((long long)M + li.tile_m - 1) / li.tile_m), p.tiles_n = (pl->N + li.tile_n - 1) / li.tile_n;
+  p.depth = li.depth, p.group = 8, p.wk = li.split;
+  p.A = reinterpret_cast<const int8_t*>(dA), p.Bt = pl->Bt, p.lda = lda, p.ldb = pl->ldb, p.ldc = ldc;
+  p.sa = dScaleA, p.sb = pl->sb, p.bias = pl->bias, p.C = dC, p.status = pl->d_status, p.timeout_ns = pl->timeout_ns;
+  p.tma_store = aligned(dC, 16) && (ldc * size) % 16 == 0;
+  WG_ON_DEVICE(pl->device);
+  CUtensorMap map_a, map_c;
+  std::memset(&map_a, 0, sizeof map_a), std::memset(&map_c, 0, sizeof map_c);
+  CUtensorMap* map_b = li.kernel == WG_INT8_TILE && li.tile_n / li.cluster == 64 ? &pl->map_b64 : &pl->map_b128;
+  if (li.kernel != WG_INT8_GEMV)
+    if ((r = encode_rows(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dA, M, pl->K, lda, li.kernel == WG_INT8_FEW ? li.tile_m : 128)) != WG_OK) return r;
+  if (li.kernel == WG_INT8_TILE && p.tma_store) {
+    const CUtensorMapDataType type = pl->out == WG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : pl->out == WG_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    if ((r = encode_rows(&map_c, type, size, dC, M, pl->N, ldc, 32)) != WG_OK) return r;
+  }
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  switch (pl->out) {
+    case WG_BF16: return I8Kernels<I8_BF16>::run(li, stream, &map_a, map_b, &map_c, &p);
+    case WG_FP16: return I8Kernels<I8_FP16>::run(li, stream, &map_a, map_b, &map_c, &p);
+    default: return I8Kernels<I8_FP32>::run(li, stream, &map_a, map_b, &map_c, &p);
+  }
+}
+
+extern "C" int wg_int8_last_device_status(void* plan, unsigned out[4]) {
+  I8Plan* pl = static_cast<I8Plan*>(plan);
+  if (!pl || !out) return WG_E_ARG;
+  WG_ON_DEVICE(pl->device);
+  WG_CUDA(cudaDeviceSynchronize());
+  WG_CUDA(cudaMemcpy(out, pl->d_status, 4 * sizeof(uint32_t), cudaMemcpyDeviceToHost));
+  return out[0] == 0 ? WG_OK : WG_E_DEVICE_WAIT;
+}
+
+extern "C" int wg_int8_plan_destroy(void* plan) {
+  I8Plan* pl = static_cast<I8Plan*>(plan);
+  if (!pl) return WG_OK;
+  DeviceGuard guard(pl->device);
+  if (pl->d_status) cudaFree(pl->d_status);
+  delete pl;
+  return WG_OK;
+}
