@@ -100,8 +100,16 @@ int encode_rows(CUtensorMap* map, CUtensorMapDataType type, int size, const void
 constexpr size_t kI8MaxSmem = 232448;
 constexpr int kI8MaxDepth = 16;
 
-// ring stages that fit beside `fixed` bytes
-int ring_depth(size_t fixed, size_t stage, int most) { return int(std::min<size_t>(size_t(most), (kI8MaxSmem - fixed) / stage)); }
+// ring rounds that fit beside `fixed` bytes
+int ring_depth(size_t fixed, size_t round, int most) { return int(std::min<size_t>(size_t(std::min(most, kI8MaxDepth)), (kI8MaxSmem - fixed) / round)); }
+
+// k-steps a round (I8Cfg)
+constexpr int kFewKsub = 2;
+constexpr int tile_ksub(int tile_m, int tile_n) { return tile_m == 256 && tile_n == 256 ? 1 : 2; }
+template <int TILE_M, int TILE_N>
+using TileCfg = I8Cfg<TILE_M / 128, TILE_N, tile_ksub(TILE_M, TILE_N)>;
+template <int TILE_M>
+using FewCfg = I8Cfg<1, TILE_M, kFewKsub>;
 
 // The launch of a named program; WG_E_VARIANT where there is none.
 int i8_derive(int M, int N, int K, wg_int8_info* o) {
@@ -118,9 +126,9 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
   if (o->kernel == WG_INT8_FEW) {
     if ((o->tile_m != 32 && o->tile_m != 64 && o->tile_m != 128) || o->tile_n != 128) return WG_E_VARIANT;
     if (o->split < 1 || o->split > 8 || o->split > kt) return WG_E_VARIANT;
-    const size_t stage = size_t(128 + o->tile_m) * 128, fixed = 1024 + sizeof(I8Ctrl) + size_t(o->split) * up(o->tile_m, o->split) * 512;
-    o->depth = ring_depth(fixed, stage, std::min(12, std::max(2, up(kt, o->split))));
-    o->dynsmem = int(fixed + o->depth * stage), o->cluster = o->split;
+    const size_t round = kFewKsub * size_t(128 + o->tile_m) * 128, fixed = 1024 + sizeof(I8Ctrl) + size_t(o->split) * up(o->tile_m, o->split) * 512;
+    o->depth = ring_depth(fixed, round, std::max(2, up(up(kt, o->split), kFewKsub)));
+    o->dynsmem = int(fixed + o->depth * round), o->cluster = o->split;
     const long long tiles = (long long)up(M, o->tile_m) * up(N, 128);
     if (tiles * o->split > 0x7fffffffll) return WG_E_LIMIT;
     o->tiles = int(tiles), o->grid = o->tiles * o->split;
@@ -130,9 +138,9 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
     const int cg = o->tile_m / 128;
     const bool known = (o->tile_m == 256 && (o->tile_n == 256 || o->tile_n == 128)) || (o->tile_m == 128 && (o->tile_n == 128 || o->tile_n == 64));
     if (!known || o->split != 1) return WG_E_VARIANT;
-    const size_t stage = size_t(128 + o->tile_n / cg) * 128, fixed = 1024 + sizeof(I8Ctrl) + 4 * 2 * 4096;
-    o->depth = ring_depth(fixed, stage, 8);
-    o->dynsmem = int(fixed + o->depth * stage), o->cluster = cg;
+    const size_t round = tile_ksub(o->tile_m, o->tile_n) * size_t(128 + o->tile_n / cg) * 128, fixed = 1024 + sizeof(I8Ctrl) + 4 * 2 * 4096;
+    o->depth = ring_depth(fixed, round, 8);
+    o->dynsmem = int(fixed + o->depth * round), o->cluster = cg;
     const long long tiles = (long long)up(M, o->tile_m) * up(N, o->tile_n);
     if (tiles > 0x3fffffffll) return WG_E_LIMIT;
     o->tiles = int(tiles), o->grid = cg * std::min(o->tiles, kSms / cg);
@@ -182,10 +190,10 @@ int launch(F* fn, const wg_int8_info& li, cudaStream_t stream, void** args) {
 template <int OUT>
 struct I8Kernels {
   static int set_up() {
-    const void* fns[] = {(const void*)i8_tile_kernel<I8Cfg<2, 256>, OUT>, (const void*)i8_tile_kernel<I8Cfg<2, 128>, OUT>,
-                         (const void*)i8_tile_kernel<I8Cfg<1, 128>, OUT>, (const void*)i8_tile_kernel<I8Cfg<1, 64>, OUT>,
-                         (const void*)i8_few_kernel<I8Cfg<1, 32>, OUT>,   (const void*)i8_few_kernel<I8Cfg<1, 64>, OUT>,
-                         (const void*)i8_few_kernel<I8Cfg<1, 128>, OUT>};
+    const void* fns[] = {(const void*)i8_tile_kernel<TileCfg<256, 256>, OUT>, (const void*)i8_tile_kernel<TileCfg<256, 128>, OUT>,
+                         (const void*)i8_tile_kernel<TileCfg<128, 128>, OUT>, (const void*)i8_tile_kernel<TileCfg<128, 64>, OUT>,
+                         (const void*)i8_few_kernel<FewCfg<32>, OUT>,   (const void*)i8_few_kernel<FewCfg<64>, OUT>,
+                         (const void*)i8_few_kernel<FewCfg<128>, OUT>};
     for (const void* fn : fns) WG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kI8MaxSmem)));
     return WG_OK;
   }
@@ -202,14 +210,14 @@ struct I8Kernels {
     if (li.kernel == WG_INT8_FEW) {
       void* args[] = {a, b, p};
       switch (li.tile_m) {
-        case 32: return launch(&i8_few_kernel<I8Cfg<1, 32>, OUT>, li, stream, args);
-        case 64: return launch(&i8_few_kernel<I8Cfg<1, 64>, OUT>, li, stream, args);
-        default: return launch(&i8_few_kernel<I8Cfg<1, 128>, OUT>, li, stream, args);
+        case 32: return launch(&i8_few_kernel<FewCfg<32>, OUT>, li, stream, args);
+        case 64: return launch(&i8_few_kernel<FewCfg<64>, OUT>, li, stream, args);
+        default: return launch(&i8_few_kernel<FewCfg<128>, OUT>, li, stream, args);
       }
     }
     void* args[] = {a, b, c, p};
-    if (li.tile_m == 256) return li.tile_n == 256 ? launch(&i8_tile_kernel<I8Cfg<2, 256>, OUT>, li, stream, args) : launch(&i8_tile_kernel<I8Cfg<2, 128>, OUT>, li, stream, args);
-    return li.tile_n == 128 ? launch(&i8_tile_kernel<I8Cfg<1, 128>, OUT>, li, stream, args) : launch(&i8_tile_kernel<I8Cfg<1, 64>, OUT>, li, stream, args);
+    if (li.tile_m == 256) return li.tile_n == 256 ? launch(&i8_tile_kernel<TileCfg<256, 256>, OUT>, li, stream, args) : launch(&i8_tile_kernel<TileCfg<256, 128>, OUT>, li, stream, args);
+    return li.tile_n == 128 ? launch(&i8_tile_kernel<TileCfg<128, 128>, OUT>, li, stream, args) : launch(&i8_tile_kernel<TileCfg<128, 64>, OUT>, li, stream, args);
   }
 };
 

@@ -28,7 +28,7 @@ struct I8Params {
   int M, N, K;           // tokens, channels, depth
   int kt;                // k-steps of 128
   int tiles_m, tiles_n;  // tiles of tokens and of channels
-  int depth;             // ring stages
+  int depth;             // ring rounds (of KSUB k-steps)
   int group;             // tile rows walked down before moving across
   int tma_store;         // Y's rows are 16-byte aligned: whole boxes go out through the copy engine
   int wk;                // gemv: warps that share a channel's K
@@ -89,31 +89,20 @@ WB_DEV bool i8_wait_warp(const I8Params& p, uint32_t abort_addr, uint32_t bar, u
 }
 
 // ---------------------------------------------------------------- kind::i8
-// D[tmem] (+)= P[smem] * Q[smem]^T: signed 8-bit operands, K-major, 32-bit sums; 32 values of K
-template <int CG>
-WB_DEV void umma_i8(uint32_t d, uint64_t pdesc, uint64_t qdesc, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CG == 2)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(pdesc),
-                 "l"(qdesc), "r"(idesc), "r"(accumulate)
-                 : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(pdesc),
-                 "l"(qdesc), "r"(idesc), "r"(accumulate)
-                 : "memory");
-}
 // instruction descriptor: 32-bit integer accumulator, both operands signed 8-bit, both K-major
 constexpr uint32_t i8_idesc(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24); }
-// operand tile: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart
-WB_DEV uint64_t i8_desc(uint32_t addr) {
-  return uint64_t((addr & 0x3FFFF) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
+// operand tiles: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart; the descriptor's low word holds the address
+constexpr uint32_t I8_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+WB_DEV uint32_t i8_desc_lo(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); }
 
 // One CTA's (pair's) operands of a tile: 128 rows of P a CTA on the accumulator's lanes, NT rows of Q as its columns.
-template <int CG_, int NT_>
+// The ring is handed over KSUB k-steps at a time (a round): a k-step of four MMAs narrower than N = 256 on a pair is shorter than
+// what its barriers, commit and bookkeeping cost the issuing thread.
+template <int CG_, int NT_, int KSUB_>
 struct I8Cfg {
-  static constexpr int CG = CG_, NT = NT_;
+  static constexpr int CG = CG_, NT = NT_, KSUB = KSUB_;
   static constexpr int Q_ROWS = NT / CG;
-  static constexpr int P_BYTES = 128 * 128, Q_BYTES = Q_ROWS * 128, STAGE = P_BYTES + Q_BYTES;
+  static constexpr int P_BYTES = 128 * 128, Q_BYTES = Q_ROWS * 128, STAGE = P_BYTES + Q_BYTES, ROUND = KSUB * STAGE;
   static constexpr uint32_t IDESC = i8_idesc(128 * CG, NT);
   static_assert(NT % 32 == 0 && NT <= 256 && Q_BYTES % 1024 == 0, "tile");
 };
@@ -124,17 +113,23 @@ WB_DEV bool i8_load(const I8Params& p, uint32_t abort_addr, uint32_t ring, uint3
                     int row_q, int kb, int ke, uint32_t& stage, uint32_t& phase) {
   const uint32_t full0 = ctrl + offsetof(I8Ctrl, full), empty0 = ctrl + offsetof(I8Ctrl, empty);
   const uint32_t full_to = C::CG == 2 ? mapa(full0, 0) : full0;
-  for (int k = kb; k < ke; ++k) {
-    if (!i8_wait_lane(p, abort_addr, empty0 + 8 * stage, phase ^ 1u, I8_WAIT_EMPTY, stage)) return false;
-    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * stage, uint32_t(C::CG * C::STAGE));
-    const uint32_t slot = ring + stage * uint32_t(C::STAGE);
-    tma_load_2d<C::CG>(slot, map_p, k * 128, row_p, full_to + 8 * stage);
-    tma_load_2d<C::CG>(slot + C::P_BYTES, map_q, k * 128, row_q, full_to + 8 * stage);
-    if (++stage == uint32_t(p.depth)) stage = 0, phase ^= 1u;
+  const uint64_t policy = l2_policy_evict_normal();
+  uint32_t left = uint32_t(ke - kb);
+  int x = kb * 128;
+  while (left != 0u) {
+    uint32_t gave_up;
+    if constexpr (C::KSUB == 1)
+      gave_up = load_k_loop<C::CG, 128>(1u, left, uint32_t(p.depth), stage, phase, x, empty0, full0, full_to, rank == 0 ? 1u : 0u, uint32_t(C::CG * C::STAGE),
+                                        ring, uint32_t(C::STAGE), uint32_t(C::P_BYTES), map_p, row_p, map_q, row_q, 1u << 14, 0u, policy);
+    else
+      gave_up = load_rounds<C::CG, C::KSUB, 128>(1u, left, uint32_t(p.depth), stage, phase, x, empty0, full0, full_to, rank == 0 ? 1u : 0u,
+                                                 uint32_t(C::CG * C::STAGE), ring, uint32_t(C::ROUND), uint32_t(C::P_BYTES), map_p, row_p, map_q, row_q,
+                                                 1u << 14, 0u, uint32_t(C::STAGE), policy);
+    if (gave_up != 0u && !i8_wait_lane(p, abort_addr, empty0 + 8 * stage, phase ^ 1u, I8_WAIT_EMPTY, stage)) return false;
   }
   return true;
 }
-// Every stage loaded has been handed back before the CTA leaves.
+// Every round loaded has been handed back before the CTA leaves.
 WB_DEV bool i8_load_done(const I8Params& p, uint32_t abort_addr, uint32_t ctrl, uint32_t stage, uint32_t phase) {
   for (int i = 0; i < p.depth; ++i) {
     if (!i8_wait_lane(p, abort_addr, ctrl + offsetof(I8Ctrl, empty) + 8 * stage, phase ^ 1u, I8_WAIT_EMPTY, 0x100u + stage)) return false;
@@ -143,27 +138,22 @@ WB_DEV bool i8_load_done(const I8Params& p, uint32_t abort_addr, uint32_t ctrl, 
   return true;
 }
 
-// MMA issuer, one lane (of the pair's leader): the commit that frees the stage before goes out after this stage's first
-// MMA, the next stage is asked for before the last, so that neither stands between two stages' MMAs.
+// MMA issuer, one lane (of the pair's leader): `left` k-steps of a tile into the accumulator at column d.
 template <class C>
-WB_DEV bool i8_mma(const I8Params& p, uint32_t abort_addr, uint32_t ring, uint32_t ctrl, uint32_t d, int steps, uint32_t& stage, uint32_t& phase) {
+WB_DEV bool i8_mma(const I8Params& p, uint32_t abort_addr, uint32_t ring, uint32_t ctrl, uint32_t d, uint32_t left, uint32_t& stage, uint32_t& phase) {
   const uint32_t full0 = ctrl + offsetof(I8Ctrl, full), empty0 = ctrl + offsetof(I8Ctrl, empty);
-  constexpr uint16_t mask = C::CG == 2 ? 0x3 : 0x1;
-  uint32_t ready = 0, before = 0;
-  for (int k = 0; k < steps; ++k) {
-    if (!ready && !i8_wait_lane(p, abort_addr, full0 + 8 * stage, phase, I8_WAIT_FULL, stage)) return false;
-    const uint32_t slot = ring + stage * uint32_t(C::STAGE);
-    const uint64_t pd = i8_desc(slot), qd = i8_desc(slot + C::P_BYTES);
-    umma_i8<C::CG>(d, pd, qd, C::IDESC, k != 0);
-    if (k != 0) umma_commit<C::CG>(before, mask);
-    before = empty0 + 8 * stage;
-    umma_i8<C::CG>(d, pd + 2, qd + 2, C::IDESC, 1);
-    if (++stage == uint32_t(p.depth)) stage = 0, phase ^= 1u;
-    umma_i8<C::CG>(d, pd + 4, qd + 4, C::IDESC, 1);
-    ready = k + 1 < steps ? mbar_test_wait(full0 + 8 * stage, phase) : 0u;
-    umma_i8<C::CG>(d, pd + 6, qd + 6, C::IDESC, 1);
+  const uint32_t p_lo = i8_desc_lo(ring), q_lo = p_lo + (C::P_BYTES >> 4);
+  uint32_t accumulate = 0;
+  while (left != 0u) {
+    uint32_t gave_up;
+    if constexpr (C::KSUB == 1)
+      gave_up = mma_k_loop<C::CG, 1, KIND_I8>(1u, left, uint32_t(p.depth), stage, phase, accumulate, full0, empty0, d, uint32_t(C::NT), p_lo, 0u, q_lo,
+                                              uint32_t(C::STAGE >> 4), I8_DESC_HI, C::IDESC, 1u << 14);
+    else
+      gave_up = mma_rounds<C::CG, C::KSUB, KIND_I8>(1u, left, uint32_t(p.depth), stage, phase, accumulate, full0, empty0, d, uint32_t(C::NT), p_lo,
+                                                    uint32_t(C::STAGE >> 4), q_lo, uint32_t(C::ROUND >> 4), I8_DESC_HI, C::IDESC, 1u << 14);
+    if (gave_up != 0u && !i8_wait_lane(p, abort_addr, full0 + 8 * stage, phase, I8_WAIT_FULL, stage)) return false;
   }
-  umma_commit<C::CG>(before, mask);
   return true;
 }
 
@@ -211,7 +201,7 @@ struct I8Tile {
   static constexpr int COPY = 32 * 128;      // 32 rows of 128 bytes
   static constexpr int STAGING = 4 * 2 * COPY;
   static constexpr int BLOCK = OUT == I8_FP32 ? 32 : 64;  // channels a copy holds
-  static constexpr size_t smem(int depth) { return 1024 + size_t(depth) * C::STAGE + STAGING + sizeof(I8Ctrl); }
+  static constexpr size_t smem(int depth) { return 1024 + size_t(depth) * C::ROUND + STAGING + sizeof(I8Ctrl); }
 };
 
 // Tile number -> (tile of tokens, tile of channels): bands of `group` token tiles, down a band before across it, so that
@@ -243,7 +233,7 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
   using T = typename I8Out<OUT>::T;
   extern __shared__ uint8_t i8_smem[];
   const uint32_t ring = (smem_u32(i8_smem) + 1023u) & ~1023u;
-  const uint32_t staging = ring + uint32_t(p.depth) * uint32_t(C::STAGE), ctrl = staging + L::STAGING;
+  const uint32_t staging = ring + uint32_t(p.depth) * uint32_t(C::ROUND), ctrl = staging + L::STAGING;
   const uint32_t abort_addr = ctrl + offsetof(I8Ctrl, abort);
   const uint32_t warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
   const uint32_t rank = C::CG == 2 ? cluster_ctarank() : 0u;
@@ -286,7 +276,7 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
       for (int tile = first; ok && tile < ntiles; tile += step) {
         ok = i8_wait_lane(p, abort_addr, ctrl + offsetof(I8Ctrl, acc_empty) + 8 * acc, acc_phase ^ 1u, I8_WAIT_ACC_EMPTY, acc);
         tc_fence_after();
-        ok = ok && i8_mma<C>(p, abort_addr, ring, ctrl, tmem + acc * C::NT, p.kt, stage, phase);
+        ok = ok && i8_mma<C>(p, abort_addr, ring, ctrl, tmem + acc * C::NT, uint32_t(p.kt), stage, phase);
         if (ok) umma_commit<C::CG>(ctrl + offsetof(I8Ctrl, acc_full) + 8 * acc, C::CG == 2 ? 0x3 : 0x1);
         if (++acc == L::NBUF) acc = 0, acc_phase ^= 1u;
       }
@@ -417,7 +407,7 @@ struct I8Few {
   static constexpr int COLS = C::NT < 32 ? 32 : C::NT;
   static constexpr int slice(int split) { return (C::NT + split - 1) / split; }  // tokens a CTA finishes
   static constexpr size_t parts(int split) { return size_t(split) * slice(split) * 512; }
-  static constexpr size_t smem(int depth, int split) { return 1024 + size_t(depth) * C::STAGE + parts(split) + sizeof(I8Ctrl); }
+  static constexpr size_t smem(int depth, int split) { return 1024 + size_t(depth) * C::ROUND + parts(split) + sizeof(I8Ctrl); }
 };
 
 template <class C, int OUT>
@@ -431,7 +421,7 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
   const int slice = (C::NT + int(split) - 1) / int(split);
   const uint32_t ring = (smem_u32(i8_smem) + 1023u) & ~1023u;
-  const uint32_t parts = ring + uint32_t(p.depth) * uint32_t(C::STAGE), ctrl = parts + split * uint32_t(slice) * 512u;
+  const uint32_t parts = ring + uint32_t(p.depth) * uint32_t(C::ROUND), ctrl = parts + split * uint32_t(slice) * 512u;
   const uint32_t abort_addr = ctrl + offsetof(I8Ctrl, abort);
   const uint32_t warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
   const int tile = int(blockIdx.x / split), tn = tile % p.tiles_n, tm = tile / p.tiles_n;
@@ -465,7 +455,7 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
   } else if (warp == 1) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0;
-      if (i8_mma<C>(p, abort_addr, ring, ctrl, tmem, ke - kb, stage, phase)) umma_commit<1>(ctrl + offsetof(I8Ctrl, acc_full), 0x1);
+      if (i8_mma<C>(p, abort_addr, ring, ctrl, tmem, uint32_t(ke - kb), stage, phase)) umma_commit<1>(ctrl + offsetof(I8Ctrl, acc_full), 0x1);
     }
     __syncwarp();
   }

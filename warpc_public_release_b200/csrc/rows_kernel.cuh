@@ -7,11 +7,15 @@
 // The norm's root is the same for the whole row, so it cancels out of q and only enters s: one pass over the row gives
 // the sum of squares and the maximum together, and q needs nothing else.
 //
-// q is exact, not "within one": t / a is formed as t * (127 / a) in 32 bits, which is off by at most 127 * 2^-24 < 8e-6 of a
-// step (the quotient's rounding; the product is inside a fused multiply-add), so its rounding can only be wrong where
-// the distance to the nearest integer is above 0.5 - 8e-6.  Vectors holding a value beyond 0.5 - 2e-5 (four in 10^5)
-// are formed again in 64 bits, where 127 t and a are exact and the quotient's rounding cannot cross a border that a
-// quotient of two 24-bit numbers has not crossed.
+// q is exact, not "within one", without 64-bit arithmetic on the way.  What can go wrong is the rounding of a quotient next
+// to half way between two integers, and values of few bits (bf16, fp16) sit exactly there all the time (t = a / 2 gives 63.5):
+//   rows of 16-bit values (quantise): 127 t is exact in 32 bits; the quotient by a reciprocal is corrected once by its
+//     remainder, which gives the exact quotient where 32 bits hold it (half way among them), and elsewhere one nearer to
+//     the true one than that is to half way (by 254 T 2^-s - (2k + 1) A being a whole multiple of 2^-s: at least 2^-s / 2A off).
+//   otherwise: t * (127 / a) inside a fused multiply-add is off by less than 8e-6, so only a value further than
+//     0.5 - 2e-5 from its integer is in doubt.  A vector with such a value takes the sign of 254 t - (2 n +- 1) a for each:
+//     next to half way the two products agree in their leading bits, so their difference is exact in 32 bits.
+// Rows whose maximum is so small or large that these products leave the range of 32 bits are divided in 64.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -126,46 +130,71 @@ struct RowSlot {
 
 // A row's maximum and how its values are divided by it.
 struct RowDiv {
-  float amax, inv, border;  // 127 / amax; the distance to an integer beyond which 32 bits do not settle the rounding
-  bool zero;                // nothing to divide by: q = 0
+  float amax, inv;
+  bool zero;   // nothing to divide by: q = 0
+  bool wide;   // divide in 64 bits
 };
 
-// max_k |t| arrives as bits: NaN and infinity are above every finite value
+// max_k |t| arrives as bits: NaN and infinity are above every finite value.  ONE: inv is 1 / amax, else 127 / amax.
+template <bool ONE>
 __device__ __forceinline__ RowDiv row_div(uint32_t amax_bits) {
   RowDiv d;
   d.amax = __uint_as_float(amax_bits);
   d.zero = amax_bits == 0u || amax_bits >= 0x7f800000u;
-  d.inv = 127.0f / d.amax;
-  d.border = d.amax < 0x1p-100f ? -1.0f : 0.5f - 2e-5f;  // 127 / amax may overflow: the whole row in 64 bits
+  d.wide = !(d.amax > 0x1p-90f && d.amax < 0x1p118f);
+  d.inv = (ONE ? 1.0f : 127.0f) / d.amax;
   return d;
 }
 
 template <int E>
+__device__ __noinline__ void row_quantise_wide(const float* t, float amax, uint32_t* b) {
+#pragma unroll 1
+  for (int e = 0; e < E; ++e) b[e] = uint32_t(int(rint(127.0 * double(t[e]) / double(amax))));
+}
+
+// SHORT: t has at most 11 bits (the first of the two ways above)
+template <int E, bool SHORT>
 __device__ __forceinline__ void row_quantise(const float* t, const RowDiv& d, uint32_t* q4) {
   constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
   uint32_t b[E];
-  float far = 0.0f;
+  if (d.wide) {
+    float c[E];
+    uint32_t n[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float r = __fmaf_rn(t[e], d.inv, MAGIC), n = __fadd_rn(r, -MAGIC);
-    b[e] = __float_as_uint(r);
-    far = fmaxf(far, fabsf(__fmaf_rn(t[e], d.inv, -n)));
-  }
-  if (!(far <= d.border)) {
-#pragma unroll 1
+    for (int e = 0; e < E; ++e) c[e] = t[e];
+    if (!d.zero) row_quantise_wide<E>(c, d.amax, n);
+#pragma unroll
+    for (int e = 0; e < E; ++e) b[e] = d.zero ? 0u : n[e];
+  } else if constexpr (SHORT) {
+#pragma unroll
     for (int e = 0; e < E; ++e) {
-      float te = t[0];
+      const float c = __fmul_rn(127.0f, t[e]), q0 = __fmul_rn(c, d.inv);
+      const float q1 = __fmaf_rn(__fmaf_rn(-q0, d.amax, c), d.inv, q0);
+      b[e] = __float_as_uint(__fadd_rn(q1, MAGIC));
+    }
+  } else {
+    float far = 0.0f;
 #pragma unroll
-      for (int i = 1; i < E; ++i) te = e == i ? t[i] : te;
-      const uint32_t n = uint32_t(int(rint(127.0 * double(te) / double(d.amax))));
+    for (int e = 0; e < E; ++e) {
+      const float r = __fmaf_rn(t[e], d.inv, MAGIC), n = __fadd_rn(r, -MAGIC);
+      b[e] = __float_as_uint(r);
+      far = fmaxf(far, fabsf(__fmaf_rn(t[e], d.inv, -n)));
+    }
+    if (far > 0.5f - 2e-5f) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) b[i] = e == i ? n : b[i];
+      for (int e = 0; e < E; ++e) {
+        const float n = __fadd_rn(__uint_as_float(b[e]), -MAGIC), off = __fmaf_rn(t[e], d.inv, -n);
+        const float side = off < 0.0f ? -1.0f : 1.0f, half = __fmaf_rn(2.0f, n, side);  // 2 x the half way point next to t
+        const float hi = __fmul_rn(half, d.amax), lo = __fmaf_rn(half, d.amax, -hi);
+        const float past = __fmul_rn(__fadd_rn(__fmaf_rn(254.0f, t[e], -hi), -lo), side);
+        if (fabsf(off) > 0.5f - 2e-5f && (past > 0.0f || (past == 0.0f && (b[e] & 1u)))) b[e] += off < 0.0f ? 0xffffffffu : 1u;
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < E / 4; ++i) {
     const uint32_t lo = __byte_perm(b[4 * i], b[4 * i + 1], 0x0040), hi = __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040);
-    q4[i] = d.zero ? 0u : __byte_perm(lo, hi, 0x5410);
+    q4[i] = __byte_perm(lo, hi, 0x5410);
   }
 }
 
@@ -187,6 +216,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
   static_assert(NORM || !RES, "the residual comes with the norm");
   using S = RowSlot<T, VEC>;
   constexpr int E = S::E;
+  constexpr bool SHORT = !NORM && sizeof(T) == 2;
   constexpr bool AHEAD = !LOOP && VPT <= 2;  // the next row's loads are out while this row is reduced
   constexpr bool KEEP_W = !LOOP && VPT <= 4;
   __shared__ float2 part[2][32];
@@ -267,7 +297,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
           for (int e = 0; e < E; ++e) f[e] *= g[e];
         }
         uint32_t q4[E / 4];
-        row_quantise<E>(f, d, q4);
+        row_quantise<E, SHORT>(f, d, q4);
         S::store_q(p.q + row * p.ldq + c, q4, v, t, nt, p.K - c);
       }
     };
@@ -289,7 +319,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
       top = __reduce_max_sync(0xffffffffu, __float_as_uint(o.y));
       buf ^= 1;
     }
-    const RowDiv d = row_div(top);
+    const RowDiv d = row_div<SHORT>(top);
     float s = d.amax / 127.0f;
     if constexpr (NORM) {
       // squares that 32 bits cannot hold (or hold with too few of them): the sum again in 64

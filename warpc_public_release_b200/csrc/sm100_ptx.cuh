@@ -454,7 +454,7 @@ WB_DEV void umma_commit_if(uint32_t issuer, uint32_t bar, uint16_t mask) {
 // commit to empty[stage].  `accumulate` is 0 until the tile's first MMA has been issued.
 #define WB_KL_MMA(G, D, A, B, PRED)                                   \
   "mov.b64 da, {" A ", %16};\n\tmov.b64 db, {" B ", %16};\n\t"        \
-  "@e tcgen05.mma.cta_group::" G ".kind::f16 [" D "], da, db, %17, " PRED ";\n\t"
+  "@e tcgen05.mma.cta_group::" G " [" D "], da, db, %17, " PRED ";\n\t"
 #define WB_KL_MMA_J(G, D, A0, J, PRED) \
   "add.u32 ta, " A0 ", " J ";\n\tadd.u32 tb, mb, " J ";\n\t" WB_KL_MMA(G, D, "ta", "tb", PRED)
 // Order inside one k-step: the commit that frees the stage BEFORE comes after the first MMA (issued while that MMA
@@ -516,22 +516,28 @@ WB_DEV void umma_commit_if(uint32_t issuer, uint32_t bar, uint16_t mask) {
     "r"(step16), "r"(debug), "r"(hi), "r"(idesc), "r"(limit)                                                \
   : "memory"
 
-template <int CG, int REPS>
+// KIND: the operands' kind, a slot's 128 bytes of K being 64 values (f16) or 128 (i8).
+enum : int { KIND_F16 = 0, KIND_I8 = 1 };
+template <int CG, int REPS, int KIND = KIND_F16>
 WB_DEV uint32_t mma_k_loop(uint32_t issuer, uint32_t& kleft, uint32_t depth, uint32_t& stage, uint32_t& phase, uint32_t& accumulate,
                            uint32_t full0, uint32_t empty0, uint32_t d, uint32_t span, uint32_t ma_lo0, uint32_t atom16, uint32_t mb_lo0,
                            uint32_t step16, uint32_t hi, uint32_t idesc, uint32_t limit, uint32_t debug = 0) {
   uint32_t status;
-  if constexpr (CG == 2 && REPS == 1) asm volatile(WB_KL_HEAD WB_KL_STEP1("2", WB_KL_COMMIT2) WB_KL_TAIL(WB_KL_COMMIT2) WB_KL_ARGS);
-  if constexpr (CG == 2 && REPS == 2) asm volatile(WB_KL_HEAD WB_KL_STEP2("2", WB_KL_COMMIT2) WB_KL_TAIL(WB_KL_COMMIT2) WB_KL_ARGS);
-  if constexpr (CG == 1 && REPS == 1) asm volatile(WB_KL_HEAD WB_KL_STEP1("1", WB_KL_COMMIT1) WB_KL_TAIL(WB_KL_COMMIT1) WB_KL_ARGS);
-  if constexpr (CG == 1 && REPS == 2) asm volatile(WB_KL_HEAD WB_KL_STEP2("1", WB_KL_COMMIT1) WB_KL_TAIL(WB_KL_COMMIT1) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 2 && REPS == 1) asm volatile(WB_KL_HEAD WB_KL_STEP1("2.kind::f16", WB_KL_COMMIT2) WB_KL_TAIL(WB_KL_COMMIT2) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 2 && REPS == 2) asm volatile(WB_KL_HEAD WB_KL_STEP2("2.kind::f16", WB_KL_COMMIT2) WB_KL_TAIL(WB_KL_COMMIT2) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 1 && REPS == 1) asm volatile(WB_KL_HEAD WB_KL_STEP1("1.kind::f16", WB_KL_COMMIT1) WB_KL_TAIL(WB_KL_COMMIT1) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 1 && REPS == 2) asm volatile(WB_KL_HEAD WB_KL_STEP2("1.kind::f16", WB_KL_COMMIT1) WB_KL_TAIL(WB_KL_COMMIT1) WB_KL_ARGS);
+  static_assert(KIND == KIND_F16 || REPS == 1, "stacked atoms are the fp16 kernel's");
+  if constexpr (KIND == KIND_I8 && CG == 2) asm volatile(WB_KL_HEAD WB_KL_STEP1("2.kind::i8", WB_KL_COMMIT2) WB_KL_TAIL(WB_KL_COMMIT2) WB_KL_ARGS);
+  if constexpr (KIND == KIND_I8 && CG == 1) asm volatile(WB_KL_HEAD WB_KL_STEP1("1.kind::i8", WB_KL_COMMIT1) WB_KL_TAIL(WB_KL_COMMIT1) WB_KL_ARGS);
   return status;
 }
 
 // Producer: for each of `kleft` k-steps wait empty[stage], (pair leader) state the pair's bytes
 // on its own full[stage], then load the A half-tile and the B^T tile of k column x into the
 // stage's slot, both completing on full_remote0 + 8*stage (the pair leader's barrier).
-template <int CG>
+// XSTEP: a slot's values of K
+template <int CG, int XSTEP = 64>
 WB_DEV uint32_t load_k_loop(uint32_t issuer, uint32_t& kleft, uint32_t depth, uint32_t& stage, uint32_t& phase, int& x, uint32_t empty0,
                             uint32_t full0, uint32_t full_remote0, uint32_t is_leader, uint32_t tx, uint32_t ring, uint32_t stage_bytes,
                             uint32_t a_bytes, const void* map_a, int a_row, const void* map_b, int col, uint32_t limit, uint32_t debug, uint64_t policy) {
@@ -553,7 +559,7 @@ WB_DEV uint32_t load_k_loop(uint32_t issuer, uint32_t& kleft, uint32_t depth, ui
   "add.u32 sb, sa, %14;\n\t"                                                                                     \
   "@e cp.async.bulk.tensor.2d" CGQ ".shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [sa], [%15, {%4, %16}], [fr], %21;\n\t" \
   "@e cp.async.bulk.tensor.2d" CGQ ".shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [sb], [%17, {%4, %18}], [fr], %21;\n\t" \
-  "add.s32 %4, %4, 64;\n\tadd.u32 %1, %1, 1;\n\tadd.u32 eb, eb, 8;\n\tadd.u32 fl, fl, 8;\n\tadd.u32 fr, fr, 8;\n\tadd.u32 sa, sa, %13;\n\t" \
+  "add.s32 %4, %4, %22;\n\tadd.u32 %1, %1, 1;\n\tadd.u32 eb, eb, 8;\n\tadd.u32 fl, fl, 8;\n\tadd.u32 fr, fr, 8;\n\tadd.u32 sa, sa, %13;\n\t" \
   "setp.eq.u32 w, %1, %6;\n\t"                                                                                   \
   "@w mov.u32 %1, 0;\n\t@w mov.u32 eb, %7;\n\t@w mov.u32 fl, %8;\n\t@w mov.u32 fr, %9;\n\t@w mov.u32 sa, %12;\n\t@w xor.b32 %2, %2, 1;\n\t" \
   "sub.u32 %3, %3, 1;\n\tsetp.ne.u32 c, %3, 0;\n\t@c bra WB_LD_LOOP;\n"                                          \
@@ -562,7 +568,7 @@ WB_DEV uint32_t load_k_loop(uint32_t issuer, uint32_t& kleft, uint32_t depth, ui
   : "=r"(status), "+r"(stage), "+r"(phase), "+r"(kleft), "+r"(x)                                                 \
   : "r"(issuer), "r"(depth), "r"(empty0), "r"(full0), "r"(full_remote0), "r"(is_leader), "r"(tx), "r"(ring), "r"(stage_bytes), \
     "r"(a_bytes), "l"(reinterpret_cast<uint64_t>(map_a)), "r"(a_row), "l"(reinterpret_cast<uint64_t>(map_b)), "r"(col), "r"(debug), "r"(limit), \
-    "l"(policy)                                                                                                  \
+    "l"(policy), "n"(XSTEP)                                                                                                  \
   : "memory"
   if constexpr (CG == 2) asm volatile(WB_LD_BODY(".cta_group::2") WB_LD_ARGS);
   else asm volatile(WB_LD_BODY("") WB_LD_ARGS);
@@ -584,7 +590,7 @@ WB_DEV uint32_t load_k_loop(uint32_t issuer, uint32_t& kleft, uint32_t depth, ui
 // rounds, step16 / stage_bytes the size of a ROUND and slot16 / slot_bytes that of one slot.
 #define WB_KR_MMA(G, D, A, B, PRED, GUARD)                            \
   "mov.b64 da, {" A ", %16};\n\tmov.b64 db, {" B ", %16};\n\t"        \
-  "@" GUARD " tcgen05.mma.cta_group::" G ".kind::f16 [" D "], da, db, %17, " PRED ";\n\t"
+  "@" GUARD " tcgen05.mma.cta_group::" G " [" D "], da, db, %17, " PRED ";\n\t"
 #define WB_KR_MMA_J(G, A0, B0, J, GUARD) \
   "add.u32 ta, " A0 ", " J ";\n\tadd.u32 tb, " B0 ", " J ";\n\t" WB_KR_MMA(G, "%9", "ta", "tb", "pt", GUARD)
 // k-step g (>= 1) of the round: its slot's descriptors, four MMAs under the guard for "it exists"
@@ -686,22 +692,26 @@ WB_DEV uint32_t load_k_loop(uint32_t issuer, uint32_t& kleft, uint32_t depth, ui
 #define WB_KR_BODY4(G, COMMIT)                                                                       \
   WB_KR_ROUND4(G, COMMIT) WB_KR_LAST_HEAD WB_KR_STEP0_LAST(G, COMMIT) WB_KR_GROUP(G, "e1") WB_KR_GROUP(G, "e2") WB_KR_GROUP(G, "e3")
 
-template <int CG, int KSUB>
+template <int CG, int KSUB, int KIND = KIND_F16>
 WB_DEV uint32_t mma_rounds(uint32_t issuer, uint32_t& kleft, uint32_t depth, uint32_t& stage, uint32_t& phase, uint32_t& accumulate,
                            uint32_t full0, uint32_t empty0, uint32_t d, uint32_t span, uint32_t ma_lo0, uint32_t atom16, uint32_t mb_lo0,
                            uint32_t step16, uint32_t hi, uint32_t idesc, uint32_t limit, uint32_t debug = 0) {
   static_assert(KSUB == 2 || KSUB == 4, "rounds of two or four k-steps");
   uint32_t status;
-  if constexpr (CG == 2 && KSUB == 2) asm volatile(WB_KR_HEAD("2") WB_KR_BODY2("2", WB_KL_COMMIT2) WB_KR_END(WB_KL_COMMIT2) WB_KL_ARGS);
-  if constexpr (CG == 2 && KSUB == 4) asm volatile(WB_KR_HEAD("4") WB_KR_BODY4("2", WB_KL_COMMIT2) WB_KR_END(WB_KL_COMMIT2) WB_KL_ARGS);
-  if constexpr (CG == 1 && KSUB == 2) asm volatile(WB_KR_HEAD("2") WB_KR_BODY2("1", WB_KL_COMMIT1) WB_KR_END(WB_KL_COMMIT1) WB_KL_ARGS);
-  if constexpr (CG == 1 && KSUB == 4) asm volatile(WB_KR_HEAD("4") WB_KR_BODY4("1", WB_KL_COMMIT1) WB_KR_END(WB_KL_COMMIT1) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 2 && KSUB == 2) asm volatile(WB_KR_HEAD("2") WB_KR_BODY2("2.kind::f16", WB_KL_COMMIT2) WB_KR_END(WB_KL_COMMIT2) WB_KL_ARGS);
+  if constexpr (KIND == KIND_I8 && CG == 2 && KSUB == 2) asm volatile(WB_KR_HEAD("2") WB_KR_BODY2("2.kind::i8", WB_KL_COMMIT2) WB_KR_END(WB_KL_COMMIT2) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 2 && KSUB == 4) asm volatile(WB_KR_HEAD("4") WB_KR_BODY4("2.kind::f16", WB_KL_COMMIT2) WB_KR_END(WB_KL_COMMIT2) WB_KL_ARGS);
+  if constexpr (KIND == KIND_I8 && CG == 2 && KSUB == 4) asm volatile(WB_KR_HEAD("4") WB_KR_BODY4("2.kind::i8", WB_KL_COMMIT2) WB_KR_END(WB_KL_COMMIT2) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 1 && KSUB == 2) asm volatile(WB_KR_HEAD("2") WB_KR_BODY2("1.kind::f16", WB_KL_COMMIT1) WB_KR_END(WB_KL_COMMIT1) WB_KL_ARGS);
+  if constexpr (KIND == KIND_I8 && CG == 1 && KSUB == 2) asm volatile(WB_KR_HEAD("2") WB_KR_BODY2("1.kind::i8", WB_KL_COMMIT1) WB_KR_END(WB_KL_COMMIT1) WB_KL_ARGS);
+  if constexpr (KIND == KIND_F16 && CG == 1 && KSUB == 4) asm volatile(WB_KR_HEAD("4") WB_KR_BODY4("1.kind::f16", WB_KL_COMMIT1) WB_KR_END(WB_KL_COMMIT1) WB_KL_ARGS);
+  if constexpr (KIND == KIND_I8 && CG == 1 && KSUB == 4) asm volatile(WB_KR_HEAD("4") WB_KR_BODY4("1.kind::i8", WB_KL_COMMIT1) WB_KR_END(WB_KL_COMMIT1) WB_KL_ARGS);
   return status;
 }
 
 // Producer, a round at a time: wait empty[round], (pair leader) state the bytes of the round's
 // k-steps that exist, load each of them into its slot.
-template <int CG, int KSUB>
+template <int CG, int KSUB, int XSTEP = 64>
 WB_DEV uint32_t load_rounds(uint32_t issuer, uint32_t& kleft, uint32_t depth, uint32_t& stage, uint32_t& phase, int& x, uint32_t empty0,
                             uint32_t full0, uint32_t full_remote0, uint32_t is_leader, uint32_t tx, uint32_t ring, uint32_t stage_bytes,
                             uint32_t a_bytes, const void* map_a, int a_row, const void* map_b, int col, uint32_t limit, uint32_t debug,
@@ -712,7 +722,7 @@ WB_DEV uint32_t load_rounds(uint32_t issuer, uint32_t& kleft, uint32_t depth, ui
   "add.u32 sb, sg, %14;\n\t"                                                                                     \
   "@" GUARD " cp.async.bulk.tensor.2d" CGQ ".shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [sg], [%15, {xg, %16}], [fr], %22;\n\t" \
   "@" GUARD " cp.async.bulk.tensor.2d" CGQ ".shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [sb], [%17, {xg, %18}], [fr], %22;\n\t" \
-  "add.u32 sg, sg, %21;\n\tadd.s32 xg, xg, 64;\n\t"
+  "add.u32 sg, sg, %21;\n\tadd.s32 xg, xg, %23;\n\t"
 #define WB_LR_BODY(CGQ, KSUB_S, MORE)                                                                            \
   "{\n\t.reg .pred e, e1, e2, e3, ei, pl, pn, p, q, w, c;\n\t.reg .b32 n, eb, fl, fr, sa, sb, sg, xg, par, dbg, use, txr;\n\t" \
   "setp.ne.u32 ei, %5, 0;\n\tand.b32 dbg, %19, 1;\n\tsetp.eq.and.u32 e, dbg, 0, ei;\n\t"                          \
@@ -731,7 +741,7 @@ WB_DEV uint32_t load_rounds(uint32_t issuer, uint32_t& kleft, uint32_t depth, ui
   "@pn mbarrier.arrive.shared::cta.b64 _, [fl];\n\t"                                                             \
   "mov.u32 sg, sa;\n\tmov.u32 xg, %4;\n\t"                                                                       \
   WB_LR_LOADS(CGQ, "e") WB_LR_LOADS(CGQ, "e1") MORE                                                              \
-  "mad.lo.s32 %4, use, 64, %4;\n\tadd.u32 %1, %1, 1;\n\tadd.u32 eb, eb, 8;\n\tadd.u32 fl, fl, 8;\n\tadd.u32 fr, fr, 8;\n\tadd.u32 sa, sa, %13;\n\t" \
+  "mad.lo.s32 %4, use, %23, %4;\n\tadd.u32 %1, %1, 1;\n\tadd.u32 eb, eb, 8;\n\tadd.u32 fl, fl, 8;\n\tadd.u32 fr, fr, 8;\n\tadd.u32 sa, sa, %13;\n\t" \
   "setp.eq.u32 w, %1, %6;\n\t"                                                                                   \
   "@w mov.u32 %1, 0;\n\t@w mov.u32 eb, %7;\n\t@w mov.u32 fl, %8;\n\t@w mov.u32 fr, %9;\n\t@w mov.u32 sa, %12;\n\t@w xor.b32 %2, %2, 1;\n\t" \
   "sub.u32 %3, %3, use;\n\tsetp.ne.u32 c, %3, 0;\n\t@c bra WB_LR_LOOP;\n"                                        \
@@ -740,7 +750,7 @@ WB_DEV uint32_t load_rounds(uint32_t issuer, uint32_t& kleft, uint32_t depth, ui
   : "=r"(status), "+r"(stage), "+r"(phase), "+r"(kleft), "+r"(x)                                                 \
   : "r"(issuer), "r"(depth), "r"(empty0), "r"(full0), "r"(full_remote0), "r"(is_leader), "r"(tx), "r"(ring), "r"(stage_bytes), \
     "r"(a_bytes), "l"(reinterpret_cast<uint64_t>(map_a)), "r"(a_row), "l"(reinterpret_cast<uint64_t>(map_b)), "r"(col), "r"(debug), "r"(limit), \
-    "r"(slot_bytes), "l"(policy)                                                                                 \
+    "r"(slot_bytes), "l"(policy), "n"(XSTEP)                                                                                 \
   : "memory"
   if constexpr (CG == 2 && KSUB == 2) asm volatile(WB_LR_BODY(".cta_group::2", "2", "") WB_LR_ARGS);
   if constexpr (CG == 2 && KSUB == 4) asm volatile(WB_LR_BODY(".cta_group::2", "4", WB_LR_LOADS(".cta_group::2", "e2") WB_LR_LOADS(".cta_group::2", "e3")) WB_LR_ARGS);
