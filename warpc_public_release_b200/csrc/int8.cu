@@ -25,33 +25,43 @@ struct RowLaunch {
   bool loop;
 };
 
-// How a row is spread: `slots` vectors of 16 bytes.  A warp a row up to 64 vectors (no barrier); else a block a row, two
-// vectors a thread while a block holds the row so (the next row's loads fit in registers beside them), one where there
-// are too few rows to fill the machine and only a row's own latency counts.
-RowLaunch row_launch(int M, int slots) {
+// How a row is spread: `slots` vectors of 16 bytes.  A warp a row up to 64 vectors (no barrier); else a block a row, one
+// vector a thread where there are too few rows to fill the machine and only a row's own latency counts, two otherwise.
+RowLaunch row_launch(int M, int slots, bool vec) {
   RowLaunch l;
   l.loop = false;
   if (slots <= 64) {
     l.vpt = slots <= 32 ? 1 : 2, l.threads = 32, l.rows = M > 4 * kSms ? 8 : 1;
   } else {
     l.rows = 1;
-    l.vpt = slots <= 1024 && M <= 2 * kSms ? 1 : slots <= 2048 ? 2 : 8;
-    if (slots > 4096) l.vpt = 4, l.loop = true;
-    l.threads = l.loop ? 512 : std::min(1024, (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32);
+    // vectors: up to 1024 threads with two each; scalar rows: 256 threads with one, two or four slots each
+    const int block = vec ? 1024 : 256;
+    l.vpt = slots <= block && (M <= 2 * kSms || !vec) ? 1 : slots <= 2 * block ? 2 : 4;
+    l.loop = slots > (vec ? 2 : 4) * block;
+    l.threads = !vec ? 256 : l.loop ? 512 : (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32;
   }
-  const int per_sm = std::max(1, 1024 / (l.threads * l.rows));
+  const int per_sm = std::max(1, (l.vpt <= 2 ? 1024 : 512) / (l.threads * l.rows));
   l.grid = std::min((M + l.rows - 1) / l.rows, kSms * per_sm);
   return l;
 }
 
 template <class T, bool NORM, bool RES, bool VEC>
 int launch_rows(const RowParams& p, cudaStream_t stream) {
-  const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E);
+  const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E, VEC);
   const dim3 block(unsigned(l.threads), unsigned(l.rows)), grid(unsigned(l.grid));
-  if (l.loop) rows_kernel<T, NORM, RES, VEC, 4, true><<<grid, block, 0, stream>>>(p);
-  else if (l.vpt == 1) rows_kernel<T, NORM, RES, VEC, 1, false><<<grid, block, 0, stream>>>(p);
-  else if (l.vpt == 2) rows_kernel<T, NORM, RES, VEC, 2, false><<<grid, block, 0, stream>>>(p);
-  else rows_kernel<T, NORM, RES, VEC, 8, false><<<grid, block, 0, stream>>>(p);
+  constexpr int NT = VEC ? 0 : 256;
+  if (!VEC && l.threads == 32) {
+    if (l.vpt == 1) rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 1, false><<<grid, block, 0, stream>>>(p);
+    else rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 2, false><<<grid, block, 0, stream>>>(p);
+  } else if (l.loop) {
+    rows_kernel<T, NORM, RES, VEC, NT, 4, true><<<grid, block, 0, stream>>>(p);
+  } else if (l.vpt == 1) {
+    rows_kernel<T, NORM, RES, VEC, NT, 1, false><<<grid, block, 0, stream>>>(p);
+  } else if (l.vpt == 2) {
+    rows_kernel<T, NORM, RES, VEC, NT, 2, false><<<grid, block, 0, stream>>>(p);
+  } else if constexpr (!VEC) {
+    rows_kernel<T, NORM, RES, VEC, NT, 4, false><<<grid, block, 0, stream>>>(p);
+  }
   return int(cudaGetLastError());
 }
 

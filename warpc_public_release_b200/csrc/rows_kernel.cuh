@@ -12,10 +12,16 @@
 //   rows of 16-bit values (quantise): 127 t is exact in 32 bits; the quotient by a reciprocal is corrected once by its
 //     remainder, which gives the exact quotient where 32 bits hold it (half way among them), and elsewhere one nearer to
 //     the true one than that is to half way (by 254 T 2^-s - (2k + 1) A being a whole multiple of 2^-s: at least 2^-s / 2A off).
-//   otherwise: t * (127 / a) inside a fused multiply-add is off by less than 8e-6, so only a value further than
-//     0.5 - 2e-5 from its integer is in doubt.  A vector with such a value takes the sign of 254 t - (2 n +- 1) a for each:
-//     next to half way the two products agree in their leading bits, so their difference is exact in 32 bits.
+//   otherwise: t times a factor just below 127 / a and t times one just above are both rounded (each in one fused
+//     multiply-add); where the two agree, so does what lies between them.  A vector in which some do not (values within
+//     6e-5 of half way) takes the sign of 254 t - (2 n +- 1) a for each value: next to half way the two products agree in
+//     their leading bits, so their difference is exact in 32 bits.
 // Rows whose maximum is so small or large that these products leave the range of 32 bits are divided in 64.
+//
+// What bounds it is memory in the end and instructions on the way: at 6.5 TB/s an SM has about 16 instruction slots a value of a
+// 16-bit row that is only read and quantised.  So the arithmetic is in pairs (f32x2), a 16-bit row's maximum is taken on the packed
+// values, what only the row's scale needs (roots, exact divisions, the sum over the warps) is left to one warp, and a thread
+// holds up to 32 values, so that the reductions are spread over them.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,158 +42,238 @@ struct RowParams {
   float eps;
 };
 
+// ---------------------------------------------------------------- pairs of 32-bit values
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void split(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// the larger of two magnitudes; NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+  return d;
+}
+
+// 16 bytes of T: pairs of 32-bit values and back; magnitudes on the packed words (`top` of a row, kept packed, NaN kept).
 template <class T>
-struct RowVec;  // 16 bytes of T, unpacked to 32 bits and back
+struct RowVec;
 template <>
 struct RowVec<__nv_bfloat16> {
   static constexpr int E = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
+  static __device__ __forceinline__ void unpack(const uint4& v, f32x2* f) {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) f[i] = pair(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
+  static __device__ __forceinline__ uint4 pack(const f32x2* f) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      float a, b;
+      split(f[i], a, b);
+      const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
       u[i] = *reinterpret_cast<const uint32_t*>(&p);
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
   }
+  static __device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t u) {
+    u &= 0x7fff7fffu;
+    const __nv_bfloat162 p = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&top), *reinterpret_cast<const __nv_bfloat162*>(&u));
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+  static __device__ __forceinline__ float larger_of(uint32_t top) { return max_nan(__uint_as_float(top << 16), __uint_as_float(top & 0xffff0000u)); }
 };
 template <>
 struct RowVec<__half> {
   static constexpr int E = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
+  static __device__ __forceinline__ void unpack(const uint4& v, f32x2* f) {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+      f[i] = pair(p.x, p.y);
     }
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
+  static __device__ __forceinline__ uint4 pack(const f32x2* f) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      float a, b;
+      split(f[i], a, b);
+      const __half2 p = __floats2half2_rn(a, b);
       u[i] = *reinterpret_cast<const uint32_t*>(&p);
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t u) {
+    u &= 0x7fff7fffu;
+    const __half2 p = __hmax2_nan(*reinterpret_cast<const __half2*>(&top), *reinterpret_cast<const __half2*>(&u));
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+  static __device__ __forceinline__ float larger_of(uint32_t top) {
+    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&top));
+    return max_nan(p.x, p.y);
   }
 };
 template <>
 struct RowVec<float> {
   static constexpr int E = 4;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
-    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  static __device__ __forceinline__ void unpack(const uint4& v, f32x2* f) {
+    f[0] = pair(__uint_as_float(v.x), __uint_as_float(v.y)), f[1] = pair(__uint_as_float(v.z), __uint_as_float(v.w));
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  static __device__ __forceinline__ uint4 pack(const f32x2* f) {
+    float a, b, c, d;
+    split(f[0], a, b), split(f[1], c, d);
+    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
   }
 };
 
 // Where a thread's values sit in its row: slot v (of E values).  VEC: one 16-byte vector; else values `nt` apart, so that
-// the lanes of a warp read neighbouring values whatever the rows' alignment.
+// the lanes of a warp read neighbouring values whatever the rows' alignment.  NT: the threads a row as a constant, or 0.
 template <class T, bool VEC>
 struct RowSlot {
   using V = RowVec<T>;
   static constexpr int E = V::E;
   static __device__ __forceinline__ int at(int v, int e, int t, int nt) { return VEC ? (v * nt + t) * E + e : (v * E + e) * nt + t; }
+  // the slot lies inside the row for every thread (scalar: asked once a slot, not once a value)
+  static __device__ __forceinline__ bool whole(int v, int t, int nt, int K) { return VEC ? at(v, E - 1, t, nt) < K : (v + 1) * E * nt <= K; }
 
   static __device__ __forceinline__ uint4 load(const T* row, int v, int t, int nt, int K) {
-    if (VEC && at(v, E - 1, t, nt) < K) return *reinterpret_cast<const uint4*>(row + at(v, 0, t, nt));
     T part[E];
+    if (whole(v, t, nt, K)) {
+      if constexpr (VEC) return *reinterpret_cast<const uint4*>(row + at(v, 0, t, nt));
 #pragma unroll
-    for (int e = 0; e < E; ++e) part[e] = at(v, e, t, nt) < K ? row[at(v, e, t, nt)] : T(0.0f);
+      for (int e = 0; e < E; ++e) part[e] = row[at(v, e, t, nt)];
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) part[e] = at(v, e, t, nt) < K ? row[at(v, e, t, nt)] : T(0.0f);
+    }
     uint4 u;
     memcpy(&u, part, 16);
     return u;
   }
   static __device__ __forceinline__ void store(T* row, const uint4& u, int v, int t, int nt, int K) {
-    if (VEC && at(v, E - 1, t, nt) < K) {
-      *reinterpret_cast<uint4*>(row + at(v, 0, t, nt)) = u;
-      return;
-    }
     T part[E];
     memcpy(part, &u, 16);
+    if (whole(v, t, nt, K)) {
+      if constexpr (VEC) {
+        *reinterpret_cast<uint4*>(row + at(v, 0, t, nt)) = u;
+      } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (at(v, e, t, nt) < K) row[at(v, e, t, nt)] = part[e];
+        for (int e = 0; e < E; ++e) row[at(v, e, t, nt)] = part[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at(v, e, t, nt) < K) row[at(v, e, t, nt)] = part[e];
+    }
   }
   static __device__ __forceinline__ void store_q(int8_t* row, const uint32_t* q4, int v, int t, int nt, int K) {
-    if (VEC && at(v, E - 1, t, nt) < K) {
-      if constexpr (E == 8) *reinterpret_cast<uint2*>(row + at(v, 0, t, nt)) = make_uint2(q4[0], q4[1]);
-      else *reinterpret_cast<uint32_t*>(row + at(v, 0, t, nt)) = q4[0];
-      return;
-    }
+    if (whole(v, t, nt, K)) {
+      if constexpr (VEC) {
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(row + at(v, 0, t, nt)) = make_uint2(q4[0], q4[1]);
+        else *reinterpret_cast<uint32_t*>(row + at(v, 0, t, nt)) = q4[0];
+      } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (at(v, e, t, nt) < K) row[at(v, e, t, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
+        for (int e = 0; e < E; ++e) row[at(v, e, t, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at(v, e, t, nt) < K) row[at(v, e, t, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
+    }
   }
 };
 
 // A row's maximum and how its values are divided by it.
 struct RowDiv {
-  float amax, inv;
-  bool zero;   // nothing to divide by: q = 0
-  bool wide;   // divide in 64 bits
+  float amax, inv;  // inv: 127 / amax, or 1 / amax where the quotient is corrected by its remainder
+  bool wide;        // zeros, values that are not finite, or too small or large for 32 bits
 };
 
-// max_k |t| arrives as bits: NaN and infinity are above every finite value.  ONE: inv is 1 / amax, else 127 / amax.
-template <bool ONE>
-__device__ __forceinline__ RowDiv row_div(uint32_t amax_bits) {
+template <bool SHORT>
+__device__ __forceinline__ RowDiv row_div(float top) {
   RowDiv d;
-  d.amax = __uint_as_float(amax_bits);
-  d.zero = amax_bits == 0u || amax_bits >= 0x7f800000u;
-  d.wide = !(d.amax > 0x1p-90f && d.amax < 0x1p118f);
-  d.inv = (ONE ? 1.0f : 127.0f) / d.amax;
+  d.amax = top;
+  d.wide = !(top > 0x1p-90f && top < 0x1p118f);  // (NaN too)
+  asm("rcp.approx.f32 %0, %1;" : "=f"(d.inv) : "f"(top));
+  if (!SHORT) d.inv *= 127.0f;
   return d;
 }
 
 template <int E>
 __device__ __noinline__ void row_quantise_wide(const float* t, float amax, uint32_t* b) {
+  const bool zero = !(amax > 0.0f) || !(amax < __int_as_float(0x7f800000));
 #pragma unroll 1
-  for (int e = 0; e < E; ++e) b[e] = uint32_t(int(rint(127.0 * double(t[e]) / double(amax))));
+  for (int e = 0; e < E; ++e) b[e] = zero ? 0u : uint32_t(int(rint(127.0 * double(t[e]) / double(amax))));
 }
 
 // SHORT: t has at most 11 bits (the first of the two ways above)
 template <int E, bool SHORT>
-__device__ __forceinline__ void row_quantise(const float* t, const RowDiv& d, uint32_t* q4) {
+__device__ __forceinline__ void row_quantise(const f32x2* t, const RowDiv& d, uint32_t* q4) {
   constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+  const f32x2 magic = pair(MAGIC, MAGIC), inv = pair(d.inv, d.inv);
   uint32_t b[E];
+  auto keep = [&](int i, f32x2 r) {
+    float x, y;
+    split(r, x, y);
+    b[2 * i] = __float_as_uint(x), b[2 * i + 1] = __float_as_uint(y);
+  };
   if (d.wide) {
     float c[E];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) split(t[i], c[2 * i], c[2 * i + 1]);
     uint32_t n[E];
+    row_quantise_wide<E>(c, d.amax, n);
 #pragma unroll
-    for (int e = 0; e < E; ++e) c[e] = t[e];
-    if (!d.zero) row_quantise_wide<E>(c, d.amax, n);
-#pragma unroll
-    for (int e = 0; e < E; ++e) b[e] = d.zero ? 0u : n[e];
+    for (int e = 0; e < E; ++e) b[e] = n[e];
   } else if constexpr (SHORT) {
+    const f32x2 c127 = pair(127.0f, 127.0f), minus = pair(-d.amax, -d.amax);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float c = __fmul_rn(127.0f, t[e]), q0 = __fmul_rn(c, d.inv);
-      const float q1 = __fmaf_rn(__fmaf_rn(-q0, d.amax, c), d.inv, q0);
-      b[e] = __float_as_uint(__fadd_rn(q1, MAGIC));
+    for (int i = 0; i < E / 2; ++i) {
+      const f32x2 c = mul2(c127, t[i]), q0 = mul2(c, inv);
+      keep(i, add2(fma2(fma2(q0, minus, c), inv, q0), magic));
     }
   } else {
-    float far = 0.0f;
+    // (the reciprocal and its product with 127 are good to 2^-22)
+    const f32x2 above = pair(d.inv * (1.0f + 0x1p-21f), d.inv * (1.0f + 0x1p-21f)), below = pair(d.inv * (1.0f - 0x1p-21f), d.inv * (1.0f - 0x1p-21f));
+    uint32_t differ = 0u;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float r = __fmaf_rn(t[e], d.inv, MAGIC), n = __fadd_rn(r, -MAGIC);
-      b[e] = __float_as_uint(r);
-      far = fmaxf(far, fabsf(__fmaf_rn(t[e], d.inv, -n)));
+    for (int i = 0; i < E / 2; ++i) {
+      keep(i, fma2(t[i], above, magic));
+      float x, y;
+      split(fma2(t[i], below, magic), x, y);
+      differ |= (__float_as_uint(x) ^ b[2 * i]) | (__float_as_uint(y) ^ b[2 * i + 1]);
     }
-    if (far > 0.5f - 2e-5f) {
+    if (differ != 0u) {
+      float c[E];
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) split(t[i], c[2 * i], c[2 * i + 1]);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float n = __fadd_rn(__uint_as_float(b[e]), -MAGIC), off = __fmaf_rn(t[e], d.inv, -n);
+        const float n = __fadd_rn(__uint_as_float(b[e]), -MAGIC), off = __fmaf_rn(c[e], d.inv, -n);
         const float side = off < 0.0f ? -1.0f : 1.0f, half = __fmaf_rn(2.0f, n, side);  // 2 x the half way point next to t
         const float hi = __fmul_rn(half, d.amax), lo = __fmaf_rn(half, d.amax, -hi);
-        const float past = __fmul_rn(__fadd_rn(__fmaf_rn(254.0f, t[e], -hi), -lo), side);
-        if (fabsf(off) > 0.5f - 2e-5f && (past > 0.0f || (past == 0.0f && (b[e] & 1u)))) b[e] += off < 0.0f ? 0xffffffffu : 1u;
+        const float past = __fmul_rn(__fadd_rn(__fmaf_rn(254.0f, c[e], -hi), -lo), side);
+        if (fabsf(off) > 0.49f && (past > 0.0f || (past == 0.0f && (b[e] & 1u)))) b[e] += off < 0.0f ? 0xffffffffu : 1u;
       }
     }
   }
@@ -209,32 +295,32 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// blockDim = (threads a row, rows a block): more than 32 threads a row only with one row a block.  VPT vectors of 16
-// bytes a thread; LOOP: rows longer than a block holds, read a second time (from L2) for the second half of the work.
-template <class T, bool NORM, bool RES, bool VEC, int VPT, bool LOOP>
+// blockDim = (threads a row, rows a block): more than 32 threads a row only with one row a block.  NT: the threads a row where
+// they are known (scalar rows: their addresses become constants), else 0.  VPT vectors of 16 bytes a thread; LOOP: rows longer
+// than a block holds, read a second time (from L2) for the second half of the work.
+template <class T, bool NORM, bool RES, bool VEC, int NT, int VPT, bool LOOP>
 __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowParams p) {
   static_assert(NORM || !RES, "the residual comes with the norm");
   using S = RowSlot<T, VEC>;
-  constexpr int E = S::E;
+  using V = typename S::V;
+  constexpr int E = S::E, P = E / 2;
   constexpr bool SHORT = !NORM && sizeof(T) == 2;
-  constexpr bool AHEAD = !LOOP && VPT <= 2;  // the next row's loads are out while this row is reduced
-  constexpr bool KEEP_W = !LOOP && VPT <= 4;
   __shared__ float2 part[2][32];
-  __shared__ double dpart[32];
-  const int t = int(threadIdx.x), nt = int(blockDim.x), lane = t & 31, warp = t >> 5, nw = nt >> 5;
+  const int t = int(threadIdx.x), nt = NT ? NT : int(blockDim.x), lane = t & 31, warp = t >> 5, nw = nt >> 5;
   const int step = int(gridDim.x * blockDim.y), chunk = nt * VPT * E;
   const T* const w = static_cast<const T*>(p.w);
   int buf = 0;
 
-  uint4 wv[KEEP_W ? VPT : 1];
-  if constexpr (NORM && KEEP_W) {
+  uint4 wv[NORM && !LOOP ? VPT : 1];
+  if constexpr (NORM && !LOOP) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) wv[v] = S::load(w, v, t, nt, p.K);
   }
-  uint4 nx[AHEAD ? VPT : 1], nr[AHEAD && RES ? VPT : 1];
+  // the next row's loads are out while this row is reduced and written
+  uint4 nx[LOOP ? 1 : VPT], nr[!LOOP && RES ? VPT : 1];
   long long row = (long long)(blockIdx.x) * blockDim.y + threadIdx.y;
   auto fetch = [&](long long i) {
-    if constexpr (AHEAD) {
+    if constexpr (!LOOP) {
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         nx[v] = S::load(static_cast<const T*>(p.x) + i * p.ldx, v, t, nt, p.K);
@@ -248,53 +334,70 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
     const T* const x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* const r = RES ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
     T* const h = RES ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
-    uint4 hv[VPT];
-    float sum = 0.0f;
-    uint32_t top = 0u;
-    // h of one chunk of the row (into registers, and out where there is a residual), its sum of squares and maximum
+    uint4 hv[SHORT && !LOOP ? VPT : 1];           // quantise, 16-bit: the values as they are
+    f32x2 tv[!SHORT && !LOOP ? VPT * P : 1];      // otherwise: t
+    f32x2 sum2 = 0ull;
+    float top = 0.0f;
+    uint32_t top2 = 0u;
+    // h of one chunk of the row (out, where there is a residual), t, the sum of squares and the maximum
     auto first = [&](int c) {
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         uint4 a;
-        if constexpr (AHEAD) a = nx[v];
-        else a = S::load(x + c, v, t, nt, p.K - c);
-        float f[E];
-        if constexpr (RES) {
-          uint4 b;
-          if constexpr (AHEAD) b = nr[v];
-          else b = S::load(r + c, v, t, nt, p.K - c);
-          float g[E];
-          S::V::unpack(a, f), S::V::unpack(b, g);
+        if constexpr (LOOP) a = S::load(x + c, v, t, nt, p.K - c);
+        else a = nx[v];
+        if constexpr (SHORT) {
+          top2 = V::larger(V::larger(top2, a.x), a.y), top2 = V::larger(V::larger(top2, a.z), a.w);
+          if constexpr (!LOOP) hv[v] = a;
+        } else {
+          f32x2 f[P];
+          V::unpack(a, f);
+          if constexpr (RES) {
+            uint4 b;
+            if constexpr (LOOP) b = S::load(r + c, v, t, nt, p.K - c);
+            else b = nr[v];
+            f32x2 g[P];
+            V::unpack(b, g);
 #pragma unroll
-          for (int e = 0; e < E; ++e) f[e] += g[e];
-          a = S::V::pack(f);
-          S::store(h + c, a, v, t, nt, p.K - c);
+            for (int i = 0; i < P; ++i) f[i] = add2(f[i], g[i]);
+            a = V::pack(f);
+            S::store(h + c, a, v, t, nt, p.K - c);
+            V::unpack(a, f);
+          }
+          if constexpr (NORM) {
+            f32x2 g[P];
+            if constexpr (LOOP) V::unpack(S::load(w + c, v, t, nt, p.K - c), g);
+            else V::unpack(wv[v], g);
+#pragma unroll
+            for (int i = 0; i < P; ++i) sum2 = fma2(f[i], f[i], sum2), f[i] = mul2(f[i], g[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            float lo, hi;
+            split(f[i], lo, hi);
+            top = max_nan(max_nan(top, lo), hi);
+            if constexpr (!LOOP) tv[v * P + i] = f[i];
+          }
         }
-        hv[v] = a;
-        S::V::unpack(a, f);
-        if constexpr (NORM) {
-          float g[E];
-          if constexpr (KEEP_W) S::V::unpack(wv[v], g);
-          else S::V::unpack(S::load(w + c, v, t, nt, p.K - c), g);
-#pragma unroll
-          for (int e = 0; e < E; ++e) sum = fmaf(f[e], f[e], sum), f[e] *= g[e];
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
       }
     };
     auto second = [&](int c, const RowDiv& d) {
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
-        float f[E];
-        if constexpr (LOOP) S::V::unpack(S::load((RES ? h : x) + c, v, t, nt, p.K - c), f);
-        else S::V::unpack(hv[v], f);
-        if constexpr (NORM) {
-          float g[E];
-          if constexpr (KEEP_W) S::V::unpack(wv[v], g);
-          else S::V::unpack(S::load(w + c, v, t, nt, p.K - c), g);
+        f32x2 f[P];
+        if constexpr (LOOP) {
+          V::unpack(S::load((RES ? h : x) + c, v, t, nt, p.K - c), f);
+          if constexpr (NORM) {
+            f32x2 g[P];
+            V::unpack(S::load(w + c, v, t, nt, p.K - c), g);
 #pragma unroll
-          for (int e = 0; e < E; ++e) f[e] *= g[e];
+            for (int i = 0; i < P; ++i) f[i] = mul2(f[i], g[i]);
+          }
+        } else if constexpr (SHORT) {
+          V::unpack(hv[v], f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < P; ++i) f[i] = tv[v * P + i];
         }
         uint32_t q4[E / 4];
         row_quantise<E, SHORT>(f, d, q4);
@@ -309,49 +412,45 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
     }
     if (row + step < p.M) fetch(row + step);
 
-    if constexpr (NORM) sum = warp_sum(sum);
-    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (SHORT) top = V::larger_of(top2);
+    // magnitudes order as their bits do, NaN above all
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    float sum = 0.0f;
+    if constexpr (NORM) {
+      float lo, hi;
+      split(sum2, lo, hi);
+      sum = warp_sum(lo + hi);
+    }
     if (nt > 32) {
-      if (lane == 0) part[buf][warp] = make_float2(sum, __uint_as_float(top));
+      if (lane == 0) part[buf][warp] = make_float2(sum, top);
       __syncthreads();
       const float2 o = lane < nw ? part[buf][lane] : make_float2(0.0f, 0.0f);
-      if constexpr (NORM) sum = warp_sum(o.x);
-      top = __reduce_max_sync(0xffffffffu, __float_as_uint(o.y));
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(o.y)));
+      if (NORM && warp == 0) sum = warp_sum(o.x);
       buf ^= 1;
     }
     const RowDiv d = row_div<SHORT>(top);
-    float s = d.amax / 127.0f;
-    if constexpr (NORM) {
-      // squares that 32 bits cannot hold (or hold with too few of them): the sum again in 64
-      if (!(sum > 0x1p-90f && sum < 0x1p126f) && !d.zero) {
-        double ds = 0.0;
-        auto squares = [&](const uint4& a) {
-          float f[E];
-          S::V::unpack(a, f);
-#pragma unroll
-          for (int e = 0; e < E; ++e) ds = fma(double(f[e]), double(f[e]), ds);
-        };
-        if constexpr (LOOP) {
-          for (int c = 0; c < p.K; c += chunk)
-            for (int v = 0; v < VPT; ++v) squares(S::load((RES ? h : x) + c, v, t, nt, p.K - c));
+    if (warp == 0) {  // the row's scale, by one warp alone
+      float s = top / 127.0f;
+      if constexpr (NORM) {
+        if (!(sum > 0x1p-90f && sum < 0x1p126f) && top > 0.0f && top < __int_as_float(0x7f800000)) {
+          // squares that 32 bits cannot hold (or hold with too few of them): the row again, in 64
+          __syncwarp();  // a warp a row: what its lanes have just written
+          double ds = 0.0;
+          const T* const again = RES ? h : x;
+          for (int i = lane; i < p.K; i += 32) {
+            const double v = double(float(again[i]));
+            ds = fma(v, v, ds);
+          }
+          s = float(double(top) / (127.0 * sqrt(warp_sum(ds) / p.K + double(p.eps))));
         } else {
-#pragma unroll
-          for (int v = 0; v < VPT; ++v) squares(hv[v]);
+          s = s / sqrtf(sum / float(p.K) + p.eps);
         }
-        ds = warp_sum(ds);
-        if (nt > 32) {
-          if (lane == 0) dpart[warp] = ds;
-          __syncthreads();
-          ds = warp_sum(lane < nw ? dpart[lane] : 0.0);
-        }
-        s = float(double(d.amax) / (127.0 * sqrt(ds / p.K + double(p.eps))));
-      } else {
-        s = s / sqrtf(sum / float(p.K) + p.eps);
       }
+      if (top == 0.0f) s = 0.0f;
+      if (!(top < __int_as_float(0x7f800000))) s = __int_as_float(0x7fc00000);
+      if (t == 0) p.scale[row] = s;
     }
-    if (top == 0u) s = 0.0f;
-    if (top >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
-    if (t == 0) p.scale[row] = s;
 
     if constexpr (LOOP) {
       for (int c = 0; c < p.K; c += chunk) second(c, d);
