@@ -79,7 +79,7 @@ def test_rule_covers_every_shape(m, n, k):
             return
     i = w.int8_choose(m, n, k)
     up = lambda a, b: -(-a // b)  # noqa: E731
-    assert i.threads == 256 and 0 <= i.dynsmem <= 232448 and 1 <= i.cluster <= 8 and i.grid % i.cluster == 0 and 0 < i.grid < 2 ** 31
+    assert i.threads in (256, 384) and 0 <= i.dynsmem <= 232448 and 1 <= i.cluster <= 8 and i.grid % i.cluster == 0 and 0 < i.grid < 2 ** 31
     if i.kernel == _lib.INT8_GEMV:
         assert m <= i.tile_m and i.tile_n * i.split == 32 and i.tiles == i.grid == up(n, i.tile_n)
     else:

@@ -148,7 +148,8 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
     const int cg = o->tile_m / 128;
     const bool known = (o->tile_m == 256 && (o->tile_n == 256 || o->tile_n == 128)) || (o->tile_m == 128 && (o->tile_n == 128 || o->tile_n == 64));
     if (!known || o->split != 1) return WG_E_VARIANT;
-    const size_t round = tile_ksub(o->tile_m, o->tile_n) * size_t(128 + o->tile_n / cg) * 128, fixed = 1024 + sizeof(I8Ctrl) + 4 * 2 * 4096;
+    const size_t round = tile_ksub(o->tile_m, o->tile_n) * size_t(128 + o->tile_n / cg) * 128, fixed = 1024 + sizeof(I8Ctrl) + (o->tile_n == 64 ? 4 : 8) * 4096;
+    o->threads = o->tile_n == 64 ? 256 : 384;
     o->depth = ring_depth(fixed, round, 8);
     o->dynsmem = int(fixed + o->depth * round), o->cluster = cg;
     const long long tiles = (long long)up(M, o->tile_m) * up(N, o->tile_n);

@@ -2,7 +2,7 @@
 //
 //   i8_tile_kernel   many tokens: a tile of tokens (accumulator lanes) x channels (columns) per CTA or CTA pair, persistent
 //   i8_few_kernel    few tokens: channels on the lanes, a tile of tokens as columns, K shared by the CTAs of a cluster
-//   i8_gemv_kernel   one to eight tokens: no tensor cores; the weights stream through the integer dot-product lanes
+//   i8_gemv_kernel   one or two tokens: no tensor cores; the weights stream through the integer dot-product lanes
 //
 // The tensor cores multiply with kind::i8 (32 values of K an instruction at the rate kind::f16 takes 16) and add in 32-bit
 // integers: exact for K <= 131071, so how K is cut or in which order the parts are added changes nothing, and every
@@ -45,6 +45,7 @@ struct I8Params {
 
 struct I8Ctrl {
   uint64_t full[16], empty[16], acc_full[2], acc_empty[2];
+  uint64_t tmem_ready;  // pair leader's: the other CTA's tensor memory is allocated
   uint32_t tmem_base, abort;
 };
 static_assert(sizeof(I8Ctrl) <= 512, "control block");
@@ -193,14 +194,19 @@ WB_DEV void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint
 }
 
 // ---------------------------------------------------------------- many tokens
-// Warps: 0 loads, 1 multiplies (and owns the tensor memory), 4-7 store; 2 and 3 only help with the set-up.
+// Warps: 0 loads, 1 multiplies (and owns the tensor memory), 2 prefetches the tensor maps, 4-11 store: two warps a quarter of the
+// accumulator's lanes, half the columns each (64 columns: one, 4-7; a tile that nothing follows is stored with nothing beside it: 2048^3, one tile a
+// pair, 14.9 -> 12.6 us against one warp a quarter; 4096 x 4096 x 1024 to fp32, 33.5 -> 23.8).
 template <class C, int OUT>
 struct I8Tile {
   static constexpr int NBUF = C::NT <= 256 ? 2 : 1;
   static constexpr int COLS = NBUF * C::NT;  // 128, 256 or 512: powers of two
   static constexpr int COPY = 32 * 128;      // 32 rows of 128 bytes
-  static constexpr int STAGING = 4 * 2 * COPY;
-  static constexpr int BLOCK = OUT == I8_FP32 ? 32 : 64;  // channels a copy holds
+  static constexpr int EPI_WARPS = C::NT == 64 ? 4 : 8, THREADS = 32 * (4 + EPI_WARPS);
+  static constexpr int STAGING = EPI_WARPS * COPY;
+  static constexpr int BLOCKS = C::NT / 32 / (EPI_WARPS / 4);  // of 32 columns, a storing warp's share of a tile
+  static constexpr int WIDTH = OUT == I8_FP32 ? 32 : 64;       // channels a copy holds
+  static_assert(BLOCKS % (WIDTH / 32) == 0, "whole copies");
   static constexpr size_t smem(int depth) { return 1024 + size_t(depth) * C::ROUND + STAGING + sizeof(I8Ctrl); }
 };
 
@@ -227,7 +233,7 @@ WB_DEV void i8_channel(const float* src, int n, int N, float* out) {
 }
 
 template <class C, int OUT>
-__global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+__global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                          const __grid_constant__ CUtensorMap map_c, const __grid_constant__ I8Params p) {
   using L = I8Tile<C, OUT>;
   using T = typename I8Out<OUT>::T;
@@ -239,23 +245,30 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
   const uint32_t rank = C::CG == 2 ? cluster_ctarank() : 0u;
   const int first = int(blockIdx.x) / C::CG, step = int(gridDim.x) / C::CG, ntiles = p.tiles_m * p.tiles_n;
 
+  // The tensor memory is allocated after the arrival: nothing needs it before the first MMA.  The storing warps learn of it
+  // at a barrier of their own, the leader's MMA lane (it writes into both CTAs') at tmem_ready.
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < p.depth; ++i) mbar_init(ctrl + offsetof(I8Ctrl, full) + 8 * i, 1), mbar_init(ctrl + offsetof(I8Ctrl, empty) + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(ctrl + offsetof(I8Ctrl, acc_full) + 8 * i, 1), mbar_init(ctrl + offsetof(I8Ctrl, acc_empty) + 8 * i, 4 * C::CG);
+    for (int i = 0; i < 2; ++i) mbar_init(ctrl + offsetof(I8Ctrl, acc_full) + 8 * i, 1), mbar_init(ctrl + offsetof(I8Ctrl, acc_empty) + 8 * i, L::EPI_WARPS * C::CG);
+    mbar_init(ctrl + offsetof(I8Ctrl, tmem_ready), 1);
     asm volatile("st.shared.u32 [%0], 0;" ::"r"(abort_addr) : "memory");
     fence_mbar_init();
   }
+  if (warp == 2 && lane == 0) prefetch_tmap(&map_a), prefetch_tmap(&map_b), prefetch_tmap(&map_c);
+  __syncwarp();
+  if constexpr (C::CG == 2) cluster_arrive_relaxed(), cluster_wait();
+  else __syncthreads();
   if (warp == 1) {
     tmem_alloc<C::CG>(ctrl + offsetof(I8Ctrl, tmem_base), L::COLS);
     tmem_relinquish<C::CG>();
+    tc_fence_before();
+    named_bar_arrive(1, 32 * (L::EPI_WARPS + 1));
+    if constexpr (C::CG == 2) mbar_arrive_cluster_relaxed_if(rank == 1 && lane == 0 ? 1u : 0u, mapa(ctrl + uint32_t(offsetof(I8Ctrl, tmem_ready)), 0));
   }
-  if (warp == 2 && lane == 0) prefetch_tmap(&map_a), prefetch_tmap(&map_b), prefetch_tmap(&map_c);
-  tc_fence_before();
-  __syncthreads();
-  if constexpr (C::CG == 2) cluster_arrive(), cluster_wait();
+  if (warp >= 4) named_bar_sync(1, 32 * (L::EPI_WARPS + 1));
   tc_fence_after();
-  uint32_t tmem;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(ctrl + uint32_t(offsetof(I8Ctrl, tmem_base))) : "memory");
+  uint32_t tmem = 0;
+  if (warp == 1 || warp >= 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(ctrl + uint32_t(offsetof(I8Ctrl, tmem_base))) : "memory");
 
   if (warp == 0) {
     if (lane == 0) {
@@ -272,7 +285,7 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-      bool ok = true;
+      bool ok = C::CG == 1 || i8_wait_lane(p, abort_addr, ctrl + offsetof(I8Ctrl, tmem_ready), 0u, I8_WAIT_ACC_EMPTY, 0x200u);
       for (int tile = first; ok && tile < ntiles; tile += step) {
         ok = i8_wait_lane(p, abort_addr, ctrl + offsetof(I8Ctrl, acc_empty) + 8 * acc, acc_phase ^ 1u, I8_WAIT_ACC_EMPTY, acc);
         tc_fence_after();
@@ -287,30 +300,32 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const uint32_t q = warp & 3u;
-    const uint32_t mine = staging + q * 2u * L::COPY;
+    const uint32_t q = warp & 3u, side = (warp - 4u) >> 2;  // which lanes, which half of the columns
+    const uint32_t copy = staging + (warp - 4u) * L::COPY, line = copy + lane * 128u, turn = lane & 7u;
     const uint32_t release = C::CG == 2 ? mapa(ctrl + uint32_t(offsetof(I8Ctrl, acc_empty)), 0) : ctrl + uint32_t(offsetof(I8Ctrl, acc_empty));
-    uint32_t acc = 0, acc_phase = 0, copies = 0;
+    constexpr int BLOCKS = L::BLOCKS;
+    uint32_t acc = 0, acc_phase = 0;
     T* const out = static_cast<T*>(p.C);
     for (int tile = first; tile < ntiles; tile += step) {
       int tm, tn;
       i8_tile_at(p, tile, tm, tn);
-      const int m0 = (tm * C::CG + int(rank)) * 128 + int(q) * 32, n0 = tn * C::NT;
+      const int m0 = (tm * C::CG + int(rank)) * 128 + int(q) * 32, n0 = tn * C::NT + int(side) * 32 * BLOCKS;
       const float sa = m0 + int(lane) < p.M ? __ldg(p.sa + m0 + lane) : 0.0f;
       if (!i8_wait_warp(p, abort_addr, ctrl + offsetof(I8Ctrl, acc_full) + 8 * acc, acc_phase, I8_WAIT_ACC_FULL, acc)) break;
       tc_fence_after();
-      const uint32_t from = tmem + acc * C::NT + (q << 21);
+      const uint32_t from = tmem + acc * C::NT + side * 32u * BLOCKS + (q << 21);
       uint32_t v[2][32];
       tmem_ld_x32(from, v[0]);
 #pragma unroll
-      for (int b = 0; b < C::NT / 32; ++b) {
+      for (int b = 0; b < BLOCKS; ++b) {
         const int n = n0 + 32 * b, half = OUT == I8_FP32 ? 0 : b & 1;
+        const bool last = b + 1 == BLOCKS;
         float s[32];
         i8_channel(p.sb, n, p.N, s);
         tmem_wait_ld();
-        if (b + 1 < C::NT / 32) {
+        if (!last) {
           tmem_ld_x32(from + 32 * (b + 1), v[(b + 1) & 1]);
-        } else {  // the accumulator is read out: the next tile but one may go there
+        } else {  // read out, as far as this warp goes: the next tile but one may have the accumulator
           tc_fence_before();
           __syncwarp();
           if constexpr (C::CG == 2) mbar_arrive_cluster_relaxed_if(lane == 0 ? 1u : 0u, release + 8 * acc);
@@ -326,9 +341,8 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
           for (int i = 0; i < 32; ++i) s[i] = i8_value(int(v[b & 1][i]), sa, s[i]);
         }
         // into a staging copy, 16-byte pieces swizzled over a row's 128 bytes (the copy engine's 128-byte swizzle)
-        const uint32_t copy = mine + (copies & 1u) * L::COPY, line = copy + lane * 128u, turn = lane & 7u;
         if (half == 0) {  // the copy's last store has been read
-          if (lane == 0) bulk_wait_read<1>();
+          if (lane == 0) bulk_wait_read<0>();
           __syncwarp();
         }
         if constexpr (OUT == I8_FP32) {
@@ -343,8 +357,7 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
                          I8Out<OUT>::two(s[8 * c + 4], s[8 * c + 5]), I8Out<OUT>::two(s[8 * c + 6], s[8 * c + 7]));
         }
         if (OUT != I8_FP32 && half == 0) continue;
-        ++copies;
-        const int nc = n0 + (OUT == I8_FP32 ? 32 * b : 32 * (b - 1));
+        const int nc = n0 + (OUT == I8_FP32 ? 32 * b : 32 * (b - half));
         if (p.tma_store) {
           fence_proxy_async_smem();
           __syncwarp();
@@ -354,12 +367,11 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
           }
         } else {  // rows of Y that the copy engine cannot write: a row at a time, neighbouring lanes neighbouring channels
           __syncwarp();
-          const uint32_t from_copy = copy;
           for (int i = 0; i < 32 && m0 + i < p.M; ++i) {
 #pragma unroll
-            for (int j = 0; j < L::BLOCK; j += 32) {
+            for (int j = 0; j < L::WIDTH; j += 32) {
               const uint32_t byte = (uint32_t(j) + lane) * uint32_t(sizeof(T));
-              const uint32_t at = from_copy + uint32_t(i) * 128u + (((byte >> 4) ^ (uint32_t(i) & 7u)) << 4) + (byte & 15u);
+              const uint32_t at = copy + uint32_t(i) * 128u + (((byte >> 4) ^ (uint32_t(i) & 7u)) << 4) + (byte & 15u);
               if (nc + j + int(lane) < p.N) {
                 T* const to = out + (long long)(m0 + i) * p.ldc + nc + j + int(lane);
                 if constexpr (OUT == I8_FP32) {
@@ -389,9 +401,11 @@ __global__ void __launch_bounds__(256, 1) i8_tile_kernel(const __grid_constant__
     while (globaltimer() - t0 < 200000ull) {
     }
   }
+  // No barrier between the pair's CTAs: every word one sends the other has been waited for by a role of the other by now (the
+  // loads that report to the leader by its MMA lane, the commits by both producers and the storing warps, the releases of the
+  // accumulators and tmem_ready by the leader's MMA lane).
   tc_fence_before();
   __syncthreads();
-  if constexpr (C::CG == 2) cluster_arrive(), cluster_wait();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<C::CG>(tmem, L::COLS);
@@ -434,17 +448,19 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
     asm volatile("st.shared.u32 [%0], 0;" ::"r"(abort_addr) : "memory");
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tmem_alloc<1>(ctrl + offsetof(I8Ctrl, tmem_base), L::COLS);
-    tmem_relinquish<1>();
-  }
   if (warp == 2 && lane == 0) prefetch_tmap(&map_a), prefetch_tmap(&map_b);
-  tc_fence_before();
   __syncthreads();
   cluster_arrive();  // every CTA of the cluster runs before another writes into its shared memory (waited for below)
+  if (warp == 1) {   // after the barrier: the first loads go out meanwhile
+    tmem_alloc<1>(ctrl + offsetof(I8Ctrl, tmem_base), L::COLS);
+    tmem_relinquish<1>();
+    tc_fence_before();
+    named_bar_arrive(1, 160);
+  }
+  if (warp >= 4) named_bar_sync(1, 160);
   tc_fence_after();
-  uint32_t tmem;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(ctrl + uint32_t(offsetof(I8Ctrl, tmem_base))) : "memory");
+  uint32_t tmem = 0;
+  if (warp == 1 || warp >= 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(ctrl + uint32_t(offsetof(I8Ctrl, tmem_base))) : "memory");
 
   if (warp == 0) {
     if (lane == 0) {
@@ -528,7 +544,7 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
   }
 }
 
-// ---------------------------------------------------------------- one to eight tokens
+// ---------------------------------------------------------------- one or two tokens
 // A warp takes R channels; its lanes take 16 bytes of K each, 512 apart; `wk` warps of the block share a channel's K.  Rows are
 // 16-byte aligned and whole 16-byte pieces are read: what a row's last piece holds past K is multiplied by zeros.
 template <int MT, int R, int OUT>
