@@ -236,7 +236,7 @@ int wg_norm_quantise_rows(int device, int M, int K, int dtype, const void* dX, l
                           void* dH, long long ldh, signed char* dQ, long long ldq, float* dScale, void* cuda_stream);
 
 /* The program of a product: WG_INT8_GEMV (tile_m >= M in {1, 2, 4, 8}; `split` warps share a channel's K), WG_INT8_FEW (tile_m
- * in {32, 64, 128} tokens x 128 channels a CTA, `split` <= 8 CTAs of a cluster share K), WG_INT8_TILE (tile_m x tile_n =
+ * in {32, 64} tokens x 128 channels a CTA, `split` in {1, 2, 4, 8} CTAs of a cluster share K), WG_INT8_TILE (tile_m x tile_n =
  * 256 x 256 or 256 x 128 on a CTA pair, 128 x 128 or 128 x 64 on a CTA; split 1). */
 enum { WG_INT8_GEMV = 1, WG_INT8_FEW = 2, WG_INT8_TILE = 3 };
 typedef struct wg_int8_info {

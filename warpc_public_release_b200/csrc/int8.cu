@@ -134,8 +134,8 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
     return WG_OK;
   }
   if (o->kernel == WG_INT8_FEW) {
-    if ((o->tile_m != 32 && o->tile_m != 64 && o->tile_m != 128) || o->tile_n != 128) return WG_E_VARIANT;
-    if (o->split < 1 || o->split > 8 || o->split > kt) return WG_E_VARIANT;
+    if ((o->tile_m != 32 && o->tile_m != 64) || o->tile_n != 128) return WG_E_VARIANT;
+    if ((o->split != 1 && o->split != 2 && o->split != 4 && o->split != 8) || o->split > kt) return WG_E_VARIANT;
     const size_t round = kFewKsub * size_t(128 + o->tile_m) * 128, fixed = 1024 + sizeof(I8Ctrl) + size_t(o->split) * up(o->tile_m, o->split) * 512;
     o->depth = ring_depth(fixed, round, std::max(2, up(up(kt, o->split), kFewKsub)));
     o->dynsmem = int(fixed + o->depth * round), o->cluster = o->split;
@@ -160,26 +160,40 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
   return WG_E_VARIANT;
 }
 
+// Which program, by estimated microseconds: what a launch costs besides its k-steps, plus its k-steps, measured on B200.
+//   gemv   2 us, and 0.21 / 0.28 / 0.45 / 0.77 us a megabyte of weights for 1 / 2 / 4 / 8 tokens (4096 x 4096: 5.5 / 6.6 / 9.4 / 14.8)
+//   few    4.9 us + 0.195 a k-step with 32 tokens, 6.4 + 0.24 with 64 (4096 x 4096: 32 k-steps 11.3, shared by two CTAs 8.0, by four
+//          6.8), 0.3 more where a cluster shares K; the weights out of memory rather than the L2 add 0.11 us a megabyte
+//   tile   per tile the slower of its k-steps and its store, the launch once (4096^3: 0.35 us a k-step with 256 x 256, 0.24 with
+//          256 x 128, 0.27 with 128 x 128, 0.21 with 128 x 64; 4096 x 4096 x 1024: a tile every 3.1, 2.3, 2.8, 2.1)
+// Clusters that run at once (a GPC holds a whole number of them): 74 of two CTAs, 32 of four, 16 of eight.
 int i8_choose(int M, int N, int K, wg_int8_info* o) {
   std::memset(o, 0, sizeof *o);
   const int kt = (K + 127) / 128;
-  auto up = [](int a, int b) { return (a + b - 1) / b; };
-  if (M <= 4) {
-    o->kernel = WG_INT8_GEMV, o->tile_m = M <= 1 ? 1 : M <= 2 ? 2 : 4, o->split = 1;
-    while (o->split < 8 && up(N, 32 / o->split) < 2 * kSms && K > 1024 * o->split) o->split *= 2;
-  } else if (M <= 128) {
-    o->kernel = WG_INT8_FEW, o->tile_m = M <= 32 ? 32 : M <= 64 ? 64 : 128, o->tile_n = 128;
-    o->split = std::max(1, std::min(std::min(8, kt), kSms / up(N, 128)));
-  } else {
-    // cycles of a wave: k-steps at the slower of the tensor pipe and the loads, and what a tile's end costs
-    static const struct { int m, n, step, end; } tiles[] = {{256, 256, 512, 5000}, {256, 128, 340, 3500}, {128, 128, 440, 3500}, {128, 64, 330, 2500}};
-    double best = 0;
-    o->kernel = WG_INT8_TILE, o->split = 1;
-    for (const auto& t : tiles) {
-      const long long n = (long long)up(M, t.m) * up(N, t.n), slots = kSms / (t.m / 128), waves = (n + slots - 1) / slots;
-      const double cost = double(waves) * kt * t.step + t.end;
-      if (best == 0 || cost < best) best = cost, o->tile_m = t.m, o->tile_n = t.n;
+  auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+  const double megabytes = double(N) * K * 1e-6;
+  double best = 1e300;
+  auto take = [&](double cost, int kernel, int tile_m, int tile_n, int split) {
+    if (cost < best) best = cost, o->kernel = kernel, o->tile_m = tile_m, o->tile_n = tile_n, o->split = split;
+  };
+  if (M <= 8) {
+    const int t = M <= 1 ? 0 : M <= 2 ? 1 : M <= 4 ? 2 : 3;
+    static const double mb[] = {0.21, 0.28, 0.45, 0.77};
+    // four channels a warp: warps enough to keep the loads of a whole machine in flight, each with 512 values of K at least
+    int wk = 1;
+    while (wk < 8 && up(N, 4) * wk < (M <= 1 ? 4096 : 2048) && K > 512 * wk) wk *= 2;
+    take(1.9 + megabytes * mb[t], WG_INT8_GEMV, 1 << t, 0, wk);
+  }
+  for (int t = 32; t <= 64; t *= 2)
+    for (int s = 1; s <= 8 && s <= kt; s *= 2) {
+      static const int at_once[] = {0, 148, 74, 0, 32, 0, 0, 0, 16};
+      const double waves = double(up(up(M, t) * up(N, 128), at_once[s]));
+      take(waves * ((t == 32 ? 4.9 : 6.4) + (t == 32 ? 0.195 : 0.24) * double(up(kt, s))) + (s > 1 ? 0.3 : 0.0) + 0.11 * megabytes, WG_INT8_FEW, t, 128, s);
     }
+  static const struct { int m, n; double launch, step, store; } tiles[] = {{256, 256, 5.8, 0.35, 3.1}, {256, 128, 4.8, 0.237, 2.3}, {128, 128, 4.6, 0.274, 2.8}, {128, 64, 4.2, 0.209, 2.1}};
+  for (const auto& t : tiles) {
+    const double each = double(up(up(M, t.m) * up(N, t.n), kSms / (t.m / 128)));
+    take(t.launch + t.step * kt + (each - 1) * std::max(t.step * kt, t.store) + 0.11 * megabytes, WG_INT8_TILE, t.m, t.n, 1);
   }
   return i8_derive(M, N, K, o);
 }
@@ -203,8 +217,7 @@ struct I8Kernels {
   static int set_up() {
     const void* fns[] = {(const void*)i8_tile_kernel<TileCfg<256, 256>, OUT>, (const void*)i8_tile_kernel<TileCfg<256, 128>, OUT>,
                          (const void*)i8_tile_kernel<TileCfg<128, 128>, OUT>, (const void*)i8_tile_kernel<TileCfg<128, 64>, OUT>,
-                         (const void*)i8_few_kernel<FewCfg<32>, OUT>,   (const void*)i8_few_kernel<FewCfg<64>, OUT>,
-                         (const void*)i8_few_kernel<FewCfg<128>, OUT>};
+                         (const void*)i8_few_kernel<FewCfg<32>, OUT>,   (const void*)i8_few_kernel<FewCfg<64>, OUT>};
     for (const void* fn : fns) WG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kI8MaxSmem)));
     return WG_OK;
   }
@@ -220,11 +233,7 @@ struct I8Kernels {
     }
     if (li.kernel == WG_INT8_FEW) {
       void* args[] = {a, b, p};
-      switch (li.tile_m) {
-        case 32: return launch(&i8_few_kernel<FewCfg<32>, OUT>, li, stream, args);
-        case 64: return launch(&i8_few_kernel<FewCfg<64>, OUT>, li, stream, args);
-        default: return launch(&i8_few_kernel<FewCfg<128>, OUT>, li, stream, args);
-      }
+      return li.tile_m == 32 ? launch(&i8_few_kernel<FewCfg<32>, OUT>, li, stream, args) : launch(&i8_few_kernel<FewCfg<64>, OUT>, li, stream, args);
     }
     void* args[] = {a, b, c, p};
     if (li.tile_m == 256) return li.tile_n == 256 ? launch(&i8_tile_kernel<TileCfg<256, 256>, OUT>, li, stream, args) : launch(&i8_tile_kernel<TileCfg<256, 128>, OUT>, li, stream, args);

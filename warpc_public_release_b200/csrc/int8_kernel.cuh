@@ -2,7 +2,7 @@
 //
 //   i8_tile_kernel   many tokens: a tile of tokens (accumulator lanes) x channels (columns) per CTA or CTA pair, persistent
 //   i8_few_kernel    few tokens: channels on the lanes, a tile of tokens as columns, K shared by the CTAs of a cluster
-//   i8_gemv_kernel   one or two tokens: no tensor cores; the weights stream through the integer dot-product lanes
+//   i8_gemv_kernel   one to eight tokens: no tensor cores; the weights stream through the integer dot-product lanes
 //
 // The tensor cores multiply with kind::i8 (32 values of K an instruction at the rate kind::f16 takes 16) and add in 32-bit
 // integers: exact for K <= 131071, so how K is cut or in which order the parts are added changes nothing, and every
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
   }
 }
 
-// ---------------------------------------------------------------- one or two tokens
+// ---------------------------------------------------------------- one to eight tokens
 // A warp takes R channels; its lanes take 16 bytes of K each, 512 apart; `wk` warps of the block share a channel's K.  Rows are
 // 16-byte aligned and whole 16-byte pieces are read: what a row's last piece holds past K is multiplied by zeros.
 template <int MT, int R, int OUT>
