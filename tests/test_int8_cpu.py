@@ -99,3 +99,13 @@ def test_rule_refuses():
 
 def test_info_layout():
     assert ctypes.sizeof(w.Int8Info) == 40
+
+
+def test_the_commands(capsys):
+    from warpc_public_release_b200 import gemm, run_int8
+    assert gemm.main(["int8", "512", "4096", "4096"]) == 0
+    line = capsys.readouterr().out
+    assert line.startswith("# int8 kernel=") and " grid=" in line
+    assert gemm.main(["int8", "0", "4096", "4096"]) == 1 and gemm.main(["int8", "5"]) == 2
+    for bad in ([], ["1", "2"], ["1", "2", "x"], ["0", "2", "3"], ["1", "2", "3", "0"], ["1", "2", "3", "--out", "int8"], ["1", "2", "3", "--out"]):
+        assert run_int8.main(bad) == 2

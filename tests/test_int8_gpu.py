@@ -514,3 +514,11 @@ def test_a_block_in_8_bits(tokens, dtype):
     block()
     torch.cuda.synchronize()
     assert torch.equal(z, first)
+
+
+@pytest.mark.parametrize("args", [["1", "300", "1111"], ["70", "260", "500", "2", "--norm"], ["300", "512", "640", "3", "--norm", "--out", "fp32"],
+                                  ["5", "64", "64", "1", "--out", "fp16"]], ids=" ".join)
+def test_the_command(args, capsys):
+    from warpc_public_release_b200 import run_int8
+    assert run_int8.main(args) == 0
+    assert " MATCH bad=0/" in capsys.readouterr().out

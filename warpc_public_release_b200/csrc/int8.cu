@@ -1,6 +1,7 @@
 // C ABI of the 8-bit operators: rows to 8 bits (with or without the root-mean-square norm before it), and the product of
 // 8-bit integers with a scale for each token and channel.
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <new>
 
@@ -45,6 +46,25 @@ RowLaunch row_launch(int M, int slots, bool vec) {
   return l;
 }
 
+// The kernel that keeps rows in shared memory (kRowRing): its limit is raised once a device.
+template <class T, bool NORM, bool RES>
+int launch_rows_ring(const RowParams& p, const RowLaunch& l, cudaStream_t stream) {
+  static std::atomic<unsigned long long> raised{0};
+  const auto kernel = &rows_kernel<T, NORM, RES, true, 0, 2, false>;
+  const size_t bytes = size_t(l.threads) * l.rows * 2 * kRowStages * 16;
+  if (bytes > 32 * 1024) {  // with the kernel's own words, 48 KB need no asking
+    int device = 0;
+    WG_CUDA(cudaGetDevice(&device));
+    const unsigned long long bit = 1ull << (device & 63);
+    if (!(raised.load() & bit)) {
+      WG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 * 2 * kRowStages * 16));
+      raised.fetch_or(bit);
+    }
+  }
+  kernel<<<dim3(unsigned(l.grid)), dim3(unsigned(l.threads), unsigned(l.rows)), bytes, stream>>>(p);
+  return int(cudaGetLastError());
+}
+
 template <class T, bool NORM, bool RES, bool VEC>
 int launch_rows(const RowParams& p, cudaStream_t stream) {
   const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E, VEC);
@@ -58,7 +78,8 @@ int launch_rows(const RowParams& p, cudaStream_t stream) {
   } else if (l.vpt == 1) {
     rows_kernel<T, NORM, RES, VEC, NT, 1, false><<<grid, block, 0, stream>>>(p);
   } else if (l.vpt == 2) {
-    rows_kernel<T, NORM, RES, VEC, NT, 2, false><<<grid, block, 0, stream>>>(p);
+    if constexpr (kRowRing<T, RES, VEC, 2, false>) return launch_rows_ring<T, NORM, RES>(p, l, stream);
+    else rows_kernel<T, NORM, RES, VEC, NT, 2, false><<<grid, block, 0, stream>>>(p);
   } else if constexpr (!VEC) {
     rows_kernel<T, NORM, RES, VEC, NT, 4, false><<<grid, block, 0, stream>>>(p);
   }

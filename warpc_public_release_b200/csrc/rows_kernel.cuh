@@ -203,6 +203,16 @@ struct RowSlot {
   }
 };
 
+// Copies of 16 bytes into shared memory that no register waits for; what lies past the row's end arrives as zeros.
+__device__ __forceinline__ void copy_ahead(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // A row's maximum and how its values are divided by it.
 struct RowDiv {
   float amax, inv;  // inv: 127 / amax, or 1 / amax where the quotient is corrected by its remainder
@@ -298,13 +308,24 @@ __device__ __forceinline__ double warp_sum(double v) {
 // blockDim = (threads a row, rows a block): more than 32 threads a row only with one row a block.  NT: the threads a row where
 // they are known (scalar rows: their addresses become constants), else 0.  VPT vectors of 16 bytes a thread; LOOP: rows longer
 // than a block holds, read a second time (from L2) for the second half of the work.
+// Vectors of 32-bit values without a residual, two a thread, have the loads of the next three rows out while one is reduced and
+// written, in slots of shared memory that only the thread itself reads (so nothing but its own copies is waited for): with the
+// next row in registers as elsewhere, 32 bytes a thread are in flight, too few at 6.5 TB/s (quantise 8192 x 8192, 65 -> 56 us).  Where
+// a residual is read too, or values have 16 bits and instructions are what is short, that is level or slower (norm with a residual
+// to 8 bits, 4096 x 8192 fp32: 72 -> 78 us; 16384 x 4096 bf16 without one: 49 -> 52; quantise 8192 x 8192 bf16: 39 both).
+constexpr int kRowStages = 4;
+template <class T, bool RES, bool VEC, int VPT, bool LOOP>
+constexpr bool kRowRing = sizeof(T) == 4 && !RES && VEC && VPT == 2 && !LOOP;
+
 template <class T, bool NORM, bool RES, bool VEC, int NT, int VPT, bool LOOP>
 __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowParams p) {
   static_assert(NORM || !RES, "the residual comes with the norm");
   using S = RowSlot<T, VEC>;
   using V = typename S::V;
   constexpr int E = S::E, P = E / 2;
-  constexpr bool SHORT = !NORM && sizeof(T) == 2;
+  constexpr bool SHORT = !NORM && sizeof(T) == 2, RING = kRowRing<T, RES, VEC, VPT, LOOP>;
+  constexpr int STAGES = kRowStages;
+  extern __shared__ uint4 row_ring[];  // [stage][v][thread]
   __shared__ float2 part[2][32];
   const int t = int(threadIdx.x), nt = NT ? NT : int(blockDim.x), lane = t & 31, warp = t >> 5, nw = nt >> 5;
   const int step = int(gridDim.x * blockDim.y), chunk = nt * VPT * E;
@@ -316,11 +337,26 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
 #pragma unroll
     for (int v = 0; v < VPT; ++v) wv[v] = S::load(w, v, t, nt, p.K);
   }
-  // the next row's loads are out while this row is reduced and written
+  // otherwise the next row's loads are out, into registers
   uint4 nx[LOOP ? 1 : VPT], nr[!LOOP && RES ? VPT : 1];
+  const int block = int(blockDim.x * blockDim.y), me = int(threadIdx.y * blockDim.x) + t;
+  auto slot = [&](int stage, int v) { return row_ring + (stage * VPT + v) * block + me; };
+  auto ahead = [&](int stage, long long i) {
+    if constexpr (RING) {
+      if (i < p.M) {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+          const int at = S::at(v, 0, t, nt), bytes = max(0, min(16, (p.K - at) * int(sizeof(T))));
+          const int from = bytes > 0 ? at : 0;
+          copy_ahead(uint32_t(__cvta_generic_to_shared(slot(stage, v))), static_cast<const T*>(p.x) + i * p.ldx + from, bytes);
+        }
+      }
+      copy_close();
+    }
+  };
   long long row = (long long)(blockIdx.x) * blockDim.y + threadIdx.y;
   auto fetch = [&](long long i) {
-    if constexpr (!LOOP) {
+    if constexpr (!LOOP && !RING) {
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         nx[v] = S::load(static_cast<const T*>(p.x) + i * p.ldx, v, t, nt, p.K);
@@ -328,9 +364,21 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
       }
     }
   };
-  if (row < p.M) fetch(row);
+  int stage = 0;
+  if constexpr (RING) {
+    for (int i = 0; i < STAGES - 1; ++i) ahead(i, row + (long long)(i) * step);
+  } else if (row < p.M) {
+    fetch(row);
+  }
 
   for (; row < p.M; row += step) {
+    if constexpr (RING) {  // the row STAGES - 1 on goes where the last one was: its values are in registers since before the barrier
+      ahead(stage == 0 ? STAGES - 1 : stage - 1, row + (long long)(STAGES - 1) * step);
+      copy_wait<STAGES - 1>();
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) nx[v] = *slot(stage, v);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
     const T* const x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* const r = RES ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
     T* const h = RES ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
@@ -410,7 +458,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
     } else {
       first(0);
     }
-    if (row + step < p.M) fetch(row + step);
+    if (!RING && row + step < p.M) fetch(row + step);
 
     if constexpr (SHORT) top = V::larger_of(top2);
     // magnitudes order as their bits do, NaN above all

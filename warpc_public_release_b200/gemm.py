@@ -3,7 +3,7 @@
 program chosen (or named) for the shape.  Exit 2 on usage, 1 where the reference's builder fails."""
 import sys
 
-from . import programs
+from . import int8, programs
 from ._lib import WarpcError
 
 USAGE = """usage: gemm [--sm sm_100a | sm_103a] <command>
@@ -11,7 +11,8 @@ USAGE = """usage: gemm [--sm sm_100a | sm_103a] <command>
        one M N K DEPTH                    one CTA a 128 x 128 tile
        pair M N K DEPTH                   CUTLASS's orientation, a 2x1 cluster
        swapped M N K TM TN DEPTH [--clc] [--ask-ahead] [--direct] [--serpentine] [--cluster-n N] [--bufs B]
-               [--group G] [--streamk] [--split S] [--split-grid S] [--split-add] [--late-launch]"""
+               [--group G] [--streamk] [--split S] [--split-grid S] [--split-add] [--late-launch]
+       int8 M N K                         the program of the 8-bit product (`# int8 key=value ...`; no reference counterpart)"""
 
 
 def build(args, sm="sm_100a"):
@@ -47,6 +48,9 @@ def main(argv=None):
             return 1
         sm, args = args[1], args[2:]
     try:
+        if len(args) == 4 and args[0] == "int8":
+            print("# int8 " + " ".join("%s=%s" % kv for kv in int8.int8_choose(*map(int, args[1:])).as_dict().items()))
+            return 0
         v, m, n, k = build(args, sm)
     except SystemExit:
         print(USAGE, file=sys.stderr)
