@@ -34,6 +34,11 @@ def test_norm_refuses(change):
     refused(WG_E_ARG, w.norm_quantise_rows, **kw)
 
 
+def test_rows_too_long():
+    refused(WG_E_LIMIT, w.quantise_rows, 1, 2 ** 30 + 1, P, P, P)
+    refused(WG_E_LIMIT, w.norm_quantise_rows, 1, 2 ** 30 + 1, P, P, 1e-6, P, P)
+
+
 def test_no_rows_is_no_work():
     w.quantise_rows(0, 64, None, None, None)
     w.norm_quantise_rows(0, 64, None, None, 1e-6, None, None)
@@ -50,7 +55,7 @@ def test_unknown_type():
 @pytest.mark.parametrize("change,code", [
     (dict(dBt=None), WG_E_ARG), (dict(dScaleB=None), WG_E_ARG), (dict(dBt=P + 8), WG_E_ARG), (dict(dScaleB=P + 4), WG_E_ARG), (dict(dBias=P + 4), WG_E_ARG),
     (dict(n=0), WG_E_ARG), (dict(k=0), WG_E_ARG), (dict(ldb=48), WG_E_ARG), (dict(ldb=72), WG_E_ARG), (dict(k=65), WG_E_ARG),
-    (dict(k=131072), WG_E_LIMIT)])
+    (dict(k=131072), WG_E_LIMIT), (dict(n=2 ** 30 + 1), WG_E_LIMIT)])
 def test_plan_refuses(change, code):
     kw = {**dict(n=64, k=64, dBt=P, dScaleB=P), **change}
     refused(code, w.Int8Plan, **kw)
@@ -66,7 +71,7 @@ def test_null_plans():
     assert l.wg_int8_plan_create(0, 64, 64, P, 64, P, None, 0, None) == WG_E_ARG
 
 
-@pytest.mark.parametrize("m", [1, 2, 3, 5, 8, 9, 17, 33, 64, 65, 128, 129, 300, 1000, 4096, 70000, 2 ** 31 - 1])
+@pytest.mark.parametrize("m", [1, 2, 3, 5, 8, 9, 17, 33, 64, 65, 128, 129, 300, 1000, 4096, 70000, 2 ** 30])
 @pytest.mark.parametrize("n", [1, 48, 1003, 4096, 16384, 100000])
 @pytest.mark.parametrize("k", [1, 100, 1111, 4096, 131071])
 def test_rule_covers_every_shape(m, n, k):
@@ -94,6 +99,8 @@ def test_rule_refuses():
     for a in ((0, 64, 64), (64, 0, 64), (64, 64, 0)):
         refused(WG_E_ARG, w.int8_choose, *a)
     refused(WG_E_LIMIT, w.int8_choose, 64, 64, 131072)
+    refused(WG_E_LIMIT, w.int8_choose, 2 ** 30 + 1, 64, 64)
+    refused(WG_E_LIMIT, w.int8_choose, 64, 2 ** 30 + 1, 64)
     assert _lib.lib().wg_int8_choose(1, 1, 1, None) == WG_E_ARG
 
 

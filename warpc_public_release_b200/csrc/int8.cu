@@ -42,7 +42,7 @@ RowLaunch row_launch(int M, int slots, bool vec) {
     l.threads = !vec ? 256 : l.loop ? 512 : (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32;
   }
   const int per_sm = std::max(1, (l.vpt <= 2 ? 1024 : 512) / (l.threads * l.rows));
-  l.grid = std::min((M + l.rows - 1) / l.rows, kSms * per_sm);
+  l.grid = int(std::min(((long long)M + l.rows - 1) / l.rows, (long long)kSms * per_sm));
   return l;
 }
 
@@ -262,13 +262,15 @@ struct I8Kernels {
   }
 };
 
-constexpr int kMaxK = 131071;  // 128 * 128 * K stays below 2^31
+constexpr int kMaxK = 131071;     // 128 * 128 * K stays below 2^31
+constexpr int kMaxSize = 1 << 30;  // tokens, channels, values a row: a tile past the end is still an int
 
 }  // namespace
 
 extern "C" int wg_quantise_rows(int device, int M, int K, int dtype, const void* dX, long long ldx, signed char* dQ, long long ldq, float* dScale,
                                 void* cuda_stream) {
   if (!known_type(dtype) || M < 0 || K <= 0 || ldx < K || ldq < K) return WG_E_ARG;
+  if (K > kMaxSize) return WG_E_LIMIT;
   if (M == 0) return WG_OK;
   if (!dX || !dQ || !dScale || !aligned(dX, unsigned(type_size(dtype))) || !aligned(dScale, 4)) return WG_E_ARG;
   RowParams p;
@@ -282,6 +284,7 @@ extern "C" int wg_norm_quantise_rows(int device, int M, int K, int dtype, const 
                                      float eps, void* dH, long long ldh, signed char* dQ, long long ldq, float* dScale, void* cuda_stream) {
   if (!known_type(dtype) || M < 0 || K <= 0 || ldx < K || ldq < K || !(eps >= 0.0f)) return WG_E_ARG;
   if ((dR == nullptr) != (dH == nullptr) || (dR && (ldr < K || ldh < K))) return WG_E_ARG;
+  if (K > kMaxSize) return WG_E_LIMIT;
   if (M == 0) return WG_OK;
   const unsigned size = unsigned(type_size(dtype));
   if (!dX || !dW || !dQ || !dScale || !aligned(dX, size) || !aligned(dW, size) || !aligned(dR, size) || !aligned(dH, size) || !aligned(dScale, 4))
@@ -298,7 +301,7 @@ extern "C" int wg_norm_quantise_rows(int device, int M, int K, int dtype, const 
 
 extern "C" int wg_int8_choose(int M, int N, int K, wg_int8_info* out) {
   if (!out || M <= 0 || N <= 0 || K <= 0) return WG_E_ARG;
-  if (K > kMaxK) return WG_E_LIMIT;
+  if (K > kMaxK || M > kMaxSize || N > kMaxSize) return WG_E_LIMIT;
   return i8_choose(M, N, K, out);
 }
 
@@ -308,7 +311,7 @@ extern "C" int wg_int8_plan_create(int device, int N, int K, const signed char* 
   *plan = nullptr;
   if (!known_type(out_dtype) || N <= 0 || K <= 0 || ldb < K || ldb % 16 != 0) return WG_E_ARG;
   if (!dBt || !dScaleB || !aligned(dBt, 16) || !aligned(dScaleB, 16) || !aligned(dBias, 16)) return WG_E_ARG;
-  if (K > kMaxK) return WG_E_LIMIT;
+  if (K > kMaxK || N > kMaxSize) return WG_E_LIMIT;
   WG_ON_DEVICE(device);
   I8Plan* pl = new (std::nothrow) I8Plan();
   if (!pl) return WG_E_ARG;
@@ -355,6 +358,7 @@ extern "C" int wg_int8_launch(void* plan, int M, const signed char* dA, long lon
   if (!pl || M < 0) return WG_E_ARG;
   const int size = type_size(pl->out);
   if (lda < pl->K || lda % 16 != 0 || ldc < pl->N) return WG_E_ARG;
+  if (M > kMaxSize) return WG_E_LIMIT;
   if (M == 0) return WG_OK;
   if (!dA || !dScaleA || !dC || !aligned(dA, 16) || !aligned(dScaleA, 4) || !aligned(dC, unsigned(size))) return WG_E_ARG;
   wg_int8_info li = pl->named;

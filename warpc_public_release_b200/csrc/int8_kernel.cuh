@@ -201,7 +201,9 @@ template <class C, int OUT>
 struct I8Tile {
   static constexpr int NBUF = C::NT <= 256 ? 2 : 1;
   static constexpr int COLS = NBUF * C::NT;  // 128, 256 or 512: powers of two
-  static constexpr int COPY = 32 * 128;      // 32 rows of 128 bytes
+  // one staging copy a warp, 32 rows of 128 bytes.  (Two, at the price of a ring stage, measured slower: 2048^3 12.6 -> 13.1 us,
+  // 4096 x 4096 x 1024 to fp32 23.8 -> 24.3, 8192^3 330-341 -> 351.)
+  static constexpr int COPY = 32 * 128;
   static constexpr int EPI_WARPS = C::NT == 64 ? 4 : 8, THREADS = 32 * (4 + EPI_WARPS);
   static constexpr int STAGING = EPI_WARPS * COPY;
   static constexpr int BLOCKS = C::NT / 32 / (EPI_WARPS / 4);  // of 32 columns, a storing warp's share of a tile
@@ -253,6 +255,7 @@ __global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(con
     mbar_init(ctrl + offsetof(I8Ctrl, tmem_ready), 1);
     asm volatile("st.shared.u32 [%0], 0;" ::"r"(abort_addr) : "memory");
     fence_mbar_init();
+    __threadfence_block();  // the abort word too, ahead of the relaxed arrival
   }
   if (warp == 2 && lane == 0) prefetch_tmap(&map_a), prefetch_tmap(&map_b), prefetch_tmap(&map_c);
   __syncwarp();
