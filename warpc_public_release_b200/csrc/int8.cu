@@ -46,18 +46,18 @@ RowLaunch row_launch(int M, int slots, bool vec) {
   return l;
 }
 
-// The kernel that keeps rows in shared memory (kRowRing): its limit is raised once a device.
+// The kernels that keep rows or weights in shared memory (kRowRing, kRowSharedW): the limit is raised once a device.
 template <class T, bool NORM, bool RES>
-int launch_rows_ring(const RowParams& p, const RowLaunch& l, cudaStream_t stream) {
+int launch_rows_shared(const RowParams& p, const RowLaunch& l, cudaStream_t stream) {
   static std::atomic<unsigned long long> raised{0};
   const auto kernel = &rows_kernel<T, NORM, RES, true, 0, 2, false>;
-  const size_t bytes = size_t(l.threads) * l.rows * 2 * kRowStages * 16;
+  const size_t bytes = size_t(l.threads) * l.rows * kRowWords<NORM> * 16;
   if (bytes > 32 * 1024) {  // with the kernel's own words, 48 KB need no asking
     int device = 0;
     WG_CUDA(cudaGetDevice(&device));
     const unsigned long long bit = 1ull << (device & 63);
     if (!(raised.load() & bit)) {
-      WG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 * 2 * kRowStages * 16));
+      WG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 * kRowWords<NORM> * 16));
       raised.fetch_or(bit);
     }
   }
@@ -66,10 +66,12 @@ int launch_rows_ring(const RowParams& p, const RowLaunch& l, cudaStream_t stream
 }
 
 template <class T, bool NORM, bool RES, bool VEC>
-int launch_rows(const RowParams& p, cudaStream_t stream) {
+int launch_rows(RowParams p, cudaStream_t stream) {
   const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E, VEC);
   const dim3 block(unsigned(l.threads), unsigned(l.rows)), grid(unsigned(l.grid));
   constexpr int NT = VEC ? 0 : 256;
+  p.step = l.grid * l.rows;
+  p.step_x = p.step * p.ldx, p.step_r = p.step * p.ldr, p.step_h = p.step * p.ldh, p.step_q = p.step * p.ldq;
   if (!VEC && l.threads == 32) {
     if (l.vpt == 1) rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 1, false><<<grid, block, 0, stream>>>(p);
     else rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 2, false><<<grid, block, 0, stream>>>(p);
@@ -78,7 +80,7 @@ int launch_rows(const RowParams& p, cudaStream_t stream) {
   } else if (l.vpt == 1) {
     rows_kernel<T, NORM, RES, VEC, NT, 1, false><<<grid, block, 0, stream>>>(p);
   } else if (l.vpt == 2) {
-    if constexpr (kRowRing<T, RES, VEC, 2, false>) return launch_rows_ring<T, NORM, RES>(p, l, stream);
+    if constexpr (VEC) return launch_rows_shared<T, NORM, RES>(p, l, stream);
     else rows_kernel<T, NORM, RES, VEC, NT, 2, false><<<grid, block, 0, stream>>>(p);
   } else if constexpr (!VEC) {
     rows_kernel<T, NORM, RES, VEC, NT, 4, false><<<grid, block, 0, stream>>>(p);

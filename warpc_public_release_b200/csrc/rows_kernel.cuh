@@ -37,7 +37,9 @@ struct RowParams {
   void* h;        // x + r as stored
   int8_t* q;
   float* scale;
-  long long ldx, ldr, ldh, ldq;  // elements between rows
+  long long ldx, ldr, ldh, ldq;                  // elements between rows
+  long long step_x, step_r, step_h, step_q;      // and between a block's (a warp's) rows: gridDim.x * blockDim.y of them
+  int step;
   int M, K;
   float eps;
 };
@@ -146,59 +148,62 @@ struct RowVec<float> {
   }
 };
 
-// Where a thread's values sit in its row: slot v (of E values).  VEC: one 16-byte vector; else values `nt` apart, so that
-// the lanes of a warp read neighbouring values whatever the rows' alignment.  NT: the threads a row as a constant, or 0.
+// Where a thread's values sit in its row: slot v (of E values) of NT threads' slots side by side.  VEC: one 16-byte vector; else
+// values `nt` apart, so that the lanes of a warp read neighbouring values whatever the rows' alignment.  `mine` points at the
+// thread's first value, `left` values of the row lie from there on (the row's own, not the thread's: the thread has every E-th
+// vector, or every nt-th value, of them).
 template <class T, bool VEC>
 struct RowSlot {
   using V = RowVec<T>;
   static constexpr int E = V::E;
-  static __device__ __forceinline__ int at(int v, int e, int t, int nt) { return VEC ? (v * nt + t) * E + e : (v * E + e) * nt + t; }
-  // the slot lies inside the row for every thread (scalar: asked once a slot, not once a value)
-  static __device__ __forceinline__ bool whole(int v, int t, int nt, int K) { return VEC ? at(v, E - 1, t, nt) < K : (v + 1) * E * nt <= K; }
+  static __device__ __forceinline__ int first(int t) { return VEC ? t * E : t; }
+  static __device__ __forceinline__ int at(int v, int e, int nt) { return VEC ? v * nt * E + e : (v * E + e) * nt; }
+  // all E values exist; scalar rows ask for all threads at once (the thread nt - 1 places on has the fewest left)
+  static __device__ __forceinline__ bool whole(int v, int t, int nt, int left) { return VEC ? at(v, E - 1, nt) < left : (v + 1) * E * nt - t <= left; }
 
-  static __device__ __forceinline__ uint4 load(const T* row, int v, int t, int nt, int K) {
+  static __device__ __forceinline__ uint4 load(const T* mine, int v, int t, int nt, int left) {
     T part[E];
-    if (whole(v, t, nt, K)) {
-      if constexpr (VEC) return *reinterpret_cast<const uint4*>(row + at(v, 0, t, nt));
+    if (whole(v, t, nt, left)) {
+      if constexpr (VEC) return *reinterpret_cast<const uint4*>(mine + at(v, 0, nt));
 #pragma unroll
-      for (int e = 0; e < E; ++e) part[e] = row[at(v, e, t, nt)];
+      for (int e = 0; e < E; ++e) part[e] = mine[at(v, e, nt)];
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) part[e] = at(v, e, t, nt) < K ? row[at(v, e, t, nt)] : T(0.0f);
+      for (int e = 0; e < E; ++e) part[e] = at(v, e, nt) < left ? mine[at(v, e, nt)] : T(0.0f);
     }
     uint4 u;
     memcpy(&u, part, 16);
     return u;
   }
-  static __device__ __forceinline__ void store(T* row, const uint4& u, int v, int t, int nt, int K) {
+  static __device__ __forceinline__ void store(T* mine, const uint4& u, int v, int t, int nt, int left) {
     T part[E];
     memcpy(part, &u, 16);
-    if (whole(v, t, nt, K)) {
+    if (whole(v, t, nt, left)) {
       if constexpr (VEC) {
-        *reinterpret_cast<uint4*>(row + at(v, 0, t, nt)) = u;
+        *reinterpret_cast<uint4*>(mine + at(v, 0, nt)) = u;
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) row[at(v, e, t, nt)] = part[e];
+        for (int e = 0; e < E; ++e) mine[at(v, e, nt)] = part[e];
       }
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (at(v, e, t, nt) < K) row[at(v, e, t, nt)] = part[e];
+        if (at(v, e, nt) < left) mine[at(v, e, nt)] = part[e];
     }
   }
-  static __device__ __forceinline__ void store_q(int8_t* row, const uint32_t* q4, int v, int t, int nt, int K) {
-    if (whole(v, t, nt, K)) {
+  static __device__ __forceinline__ void store_q(int8_t* mine, const uint32_t* q4, int v, int t, int nt, int left) {
+    if (whole(v, t, nt, left)) {
       if constexpr (VEC) {
-        if constexpr (E == 8) *reinterpret_cast<uint2*>(row + at(v, 0, t, nt)) = make_uint2(q4[0], q4[1]);
-        else *reinterpret_cast<uint32_t*>(row + at(v, 0, t, nt)) = q4[0];
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(mine + at(v, 0, nt)) = make_uint2(q4[0], q4[1]);
+        else *reinterpret_cast<uint32_t*>(mine + at(v, 0, nt)) = q4[0];
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) row[at(v, e, t, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
+        for (int e = 0; e < E; ++e) mine[at(v, e, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
       }
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (at(v, e, t, nt) < K) row[at(v, e, t, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
+        if (at(v, e, nt) < left) mine[at(v, e, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
     }
   }
 };
@@ -224,7 +229,7 @@ __device__ __forceinline__ RowDiv row_div(float top) {
   RowDiv d;
   d.amax = top;
   d.wide = !(top > 0x1p-90f && top < 0x1p118f);  // (NaN too)
-  asm("rcp.approx.f32 %0, %1;" : "=f"(d.inv) : "f"(top));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d.inv) : "f"(top));
   if (!SHORT) d.inv *= 127.0f;
   return d;
 }
@@ -308,14 +313,19 @@ __device__ __forceinline__ double warp_sum(double v) {
 // blockDim = (threads a row, rows a block): more than 32 threads a row only with one row a block.  NT: the threads a row where
 // they are known (scalar rows: their addresses become constants), else 0.  VPT vectors of 16 bytes a thread; LOOP: rows longer
 // than a block holds, read a second time (from L2) for the second half of the work.
-// Vectors of 32-bit values without a residual, two a thread, have the loads of the next three rows out while one is reduced and
-// written, in slots of shared memory that only the thread itself reads (so nothing but its own copies is waited for): with the
-// next row in registers as elsewhere, 32 bytes a thread are in flight, too few at 6.5 TB/s (quantise 8192 x 8192, 65 -> 56 us).  Where
-// a residual is read too, or values have 16 bits and instructions are what is short, that is level or slower (norm with a residual
-// to 8 bits, 4096 x 8192 fp32: 72 -> 78 us; 16384 x 4096 bf16 without one: 49 -> 52; quantise 8192 x 8192 bf16: 39 both).
+// RING: rows of vectors that are only quantised have the loads of the next three rows out while one is reduced and written, in
+// slots of shared memory that only the thread itself reads (so nothing but its own copies is waited for): with the next row in
+// registers, 32 bytes a thread are in flight, too few at 6.5 TB/s (8192 x 8192, fp32 56 -> 50.5 us = 6.6 TB/s, bf16 38 -> 33.6).  With the
+// norm that measured slower (16384 x 4096 bf16 45.1 -> 49.4 us, with a residual 84.7 -> 87.4; 4096 x 8192 fp32 69 -> 75): what is
+// short there is instructions and registers.  SHARED_W: the norm's weights, the same for all of a block's rows, in such slots too:
+// two loads a row instead of eight registers held (49 -> 45.1, fp32 71.9 -> 69.3, 40.9 -> 34.4 without a residual).
 constexpr int kRowStages = 4;
-template <class T, bool RES, bool VEC, int VPT, bool LOOP>
-constexpr bool kRowRing = sizeof(T) == 4 && !RES && VEC && VPT == 2 && !LOOP;
+template <bool NORM, bool VEC, int VPT, bool LOOP>
+constexpr bool kRowRing = !NORM && VEC && VPT == 2 && !LOOP;
+template <bool NORM, bool VEC, int VPT, bool LOOP>
+constexpr bool kRowSharedW = NORM && VEC && VPT == 2 && !LOOP;
+template <bool NORM>  // 16-byte words of shared memory a thread of these kernels
+constexpr int kRowWords = 2 * (NORM ? 1 : kRowStages);
 
 template <class T, bool NORM, bool RES, bool VEC, int NT, int VPT, bool LOOP>
 __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowParams p) {
@@ -323,65 +333,74 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
   using S = RowSlot<T, VEC>;
   using V = typename S::V;
   constexpr int E = S::E, P = E / 2;
-  constexpr bool SHORT = !NORM && sizeof(T) == 2, RING = kRowRing<T, RES, VEC, VPT, LOOP>;
+  constexpr bool SHORT = !NORM && sizeof(T) == 2, RING = kRowRing<NORM, VEC, VPT, LOOP>, SHARED_W = kRowSharedW<NORM, VEC, VPT, LOOP>;
   constexpr int STAGES = kRowStages;
-  extern __shared__ uint4 row_ring[];  // [stage][v][thread]
+  extern __shared__ uint4 row_slots[];  // RING: [stage][v][thread]; SHARED_W: [v][thread]
   __shared__ float2 part[2][32];
   const int t = int(threadIdx.x), nt = NT ? NT : int(blockDim.x), lane = t & 31, warp = t >> 5, nw = nt >> 5;
-  const int step = int(gridDim.x * blockDim.y), chunk = nt * VPT * E;
-  const T* const w = static_cast<const T*>(p.w);
+  const int chunk = nt * VPT * E, left = p.K - S::first(t);
+  const T* const w = static_cast<const T*>(p.w) + S::first(t);
   int buf = 0;
 
-  uint4 wv[NORM && !LOOP ? VPT : 1];
+  const int block = int(blockDim.x * blockDim.y), me = int(threadIdx.y * blockDim.x) + t;
+  auto slot = [&](int stage, int v) { return row_slots + (stage * VPT + v) * block + me; };
+  uint4 wv[NORM && !LOOP && !SHARED_W ? VPT : 1];
   if constexpr (NORM && !LOOP) {
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) wv[v] = S::load(w, v, t, nt, p.K);
+    for (int v = 0; v < VPT; ++v) {
+      if constexpr (SHARED_W) *slot(0, v) = S::load(w, v, t, nt, left);
+      else wv[v] = S::load(w, v, t, nt, left);
+    }
   }
+  long long row = (long long)(blockIdx.x) * blockDim.y + threadIdx.y;
+  // this thread's place in the row (in the next one to be fetched, where rows are fetched ahead), moved on row by row
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx + S::first(t);
+  const T* r = RES ? static_cast<const T*>(p.r) + row * p.ldr + S::first(t) : nullptr;
+  T* h = RES ? static_cast<T*>(p.h) + row * p.ldh + S::first(t) : nullptr;
+  int8_t* q = p.q + row * p.ldq + S::first(t);
+
   // otherwise the next row's loads are out, into registers
   uint4 nx[LOOP ? 1 : VPT], nr[!LOOP && RES ? VPT : 1];
-  const int block = int(blockDim.x * blockDim.y), me = int(threadIdx.y * blockDim.x) + t;
-  auto slot = [&](int stage, int v) { return row_ring + (stage * VPT + v) * block + me; };
-  auto ahead = [&](int stage, long long i) {
+  auto ahead = [&](int stage, bool there) {
     if constexpr (RING) {
-      if (i < p.M) {
+      if (there) {
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-          const int at = S::at(v, 0, t, nt), bytes = max(0, min(16, (p.K - at) * int(sizeof(T))));
-          const int from = bytes > 0 ? at : 0;
-          copy_ahead(uint32_t(__cvta_generic_to_shared(slot(stage, v))), static_cast<const T*>(p.x) + i * p.ldx + from, bytes);
+          const int at = S::at(v, 0, nt), bytes = max(0, min(16, (left - at) * int(sizeof(T))));
+          // (nothing left: a copy of no bytes, from the row's own memory all the same)
+          copy_ahead(uint32_t(__cvta_generic_to_shared(slot(stage, v))), bytes > 0 ? x + at : x - S::first(t), bytes);
         }
+        x += p.step_x;
       }
       copy_close();
     }
   };
-  long long row = (long long)(blockIdx.x) * blockDim.y + threadIdx.y;
-  auto fetch = [&](long long i) {
+  auto fetch = [&]() {
     if constexpr (!LOOP && !RING) {
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
-        nx[v] = S::load(static_cast<const T*>(p.x) + i * p.ldx, v, t, nt, p.K);
-        if constexpr (RES) nr[v] = S::load(static_cast<const T*>(p.r) + i * p.ldr, v, t, nt, p.K);
+        nx[v] = S::load(x, v, t, nt, left);
+        if constexpr (RES) nr[v] = S::load(r, v, t, nt, left);
       }
+      x += p.step_x;
+      if constexpr (RES) r += p.step_r;
     }
   };
   int stage = 0;
   if constexpr (RING) {
-    for (int i = 0; i < STAGES - 1; ++i) ahead(i, row + (long long)(i) * step);
+    for (int i = 0; i < STAGES - 1; ++i) ahead(i, row + (long long)(i) * p.step < p.M);
   } else if (row < p.M) {
-    fetch(row);
+    fetch();
   }
 
-  for (; row < p.M; row += step) {
+  for (; row < p.M; row += p.step) {
     if constexpr (RING) {  // the row STAGES - 1 on goes where the last one was: its values are in registers since before the barrier
-      ahead(stage == 0 ? STAGES - 1 : stage - 1, row + (long long)(STAGES - 1) * step);
+      ahead(stage == 0 ? STAGES - 1 : stage - 1, row + (long long)(STAGES - 1) * p.step < p.M);
       copy_wait<STAGES - 1>();
 #pragma unroll
       for (int v = 0; v < VPT; ++v) nx[v] = *slot(stage, v);
       stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
-    const T* const x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* const r = RES ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
-    T* const h = RES ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
     uint4 hv[SHORT && !LOOP ? VPT : 1];           // quantise, 16-bit: the values as they are
     f32x2 tv[!SHORT && !LOOP ? VPT * P : 1];      // otherwise: t
     f32x2 sum2 = 0ull;
@@ -392,7 +411,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         uint4 a;
-        if constexpr (LOOP) a = S::load(x + c, v, t, nt, p.K - c);
+        if constexpr (LOOP) a = S::load(x + c, v, t, nt, left - c);
         else a = nx[v];
         if constexpr (SHORT) {
           top2 = V::larger(V::larger(top2, a.x), a.y), top2 = V::larger(V::larger(top2, a.z), a.w);
@@ -402,19 +421,20 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
           V::unpack(a, f);
           if constexpr (RES) {
             uint4 b;
-            if constexpr (LOOP) b = S::load(r + c, v, t, nt, p.K - c);
+            if constexpr (LOOP) b = S::load(r + c, v, t, nt, left - c);
             else b = nr[v];
             f32x2 g[P];
             V::unpack(b, g);
 #pragma unroll
             for (int i = 0; i < P; ++i) f[i] = add2(f[i], g[i]);
             a = V::pack(f);
-            S::store(h + c, a, v, t, nt, p.K - c);
+            S::store(h + c, a, v, t, nt, left - c);
             V::unpack(a, f);
           }
           if constexpr (NORM) {
             f32x2 g[P];
-            if constexpr (LOOP) V::unpack(S::load(w + c, v, t, nt, p.K - c), g);
+            if constexpr (LOOP) V::unpack(S::load(w + c, v, t, nt, left - c), g);
+            else if constexpr (SHARED_W) V::unpack(*slot(0, v), g);
             else V::unpack(wv[v], g);
 #pragma unroll
             for (int i = 0; i < P; ++i) sum2 = fma2(f[i], f[i], sum2), f[i] = mul2(f[i], g[i]);
@@ -434,10 +454,10 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
       for (int v = 0; v < VPT; ++v) {
         f32x2 f[P];
         if constexpr (LOOP) {
-          V::unpack(S::load((RES ? h : x) + c, v, t, nt, p.K - c), f);
+          V::unpack(S::load((RES ? h : x) + c, v, t, nt, left - c), f);
           if constexpr (NORM) {
             f32x2 g[P];
-            V::unpack(S::load(w + c, v, t, nt, p.K - c), g);
+            V::unpack(S::load(w + c, v, t, nt, left - c), g);
 #pragma unroll
             for (int i = 0; i < P; ++i) f[i] = mul2(f[i], g[i]);
           }
@@ -449,7 +469,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
         }
         uint32_t q4[E / 4];
         row_quantise<E, SHORT>(f, d, q4);
-        S::store_q(p.q + row * p.ldq + c, q4, v, t, nt, p.K - c);
+        S::store_q(q + c, q4, v, t, nt, left - c);
       }
     };
 
@@ -458,7 +478,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
     } else {
       first(0);
     }
-    if (!RING && row + step < p.M) fetch(row + step);
+    if (!LOOP && !RING && row + p.step < p.M) fetch();
 
     if constexpr (SHORT) top = V::larger_of(top2);
     // magnitudes order as their bits do, NaN above all
@@ -485,7 +505,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
           // squares that 32 bits cannot hold (or hold with too few of them): the row again, in 64
           __syncwarp();  // a warp a row: what its lanes have just written
           double ds = 0.0;
-          const T* const again = RES ? h : x;
+          const T* const again = RES ? h - S::first(t) : static_cast<const T*>(p.x) + row * p.ldx;
           for (int i = lane; i < p.K; i += 32) {
             const double v = double(float(again[i]));
             ds = fma(v, v, ds);
@@ -502,9 +522,13 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
 
     if constexpr (LOOP) {
       for (int c = 0; c < p.K; c += chunk) second(c, d);
+      x += p.step_x;
+      if constexpr (RES) r += p.step_r;
     } else {
       second(0, d);
     }
+    if constexpr (RES) h += p.step_h;
+    q += p.step_q;
   }
 }
 
