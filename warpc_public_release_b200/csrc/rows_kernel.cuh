@@ -162,9 +162,11 @@ struct RowSlot {
   static __device__ __forceinline__ bool whole(int v, int t, int nt, int left) { return VEC ? at(v, E - 1, nt) < left : (v + 1) * E * nt - t <= left; }
 
   static __device__ __forceinline__ uint4 load(const T* mine, int v, int t, int nt, int left) {
+    if constexpr (VEC) {
+      if (whole(v, t, nt, left)) return *reinterpret_cast<const uint4*>(mine + at(v, 0, nt));
+    }
     T part[E];
-    if (whole(v, t, nt, left)) {
-      if constexpr (VEC) return *reinterpret_cast<const uint4*>(mine + at(v, 0, nt));
+    if (!VEC && whole(v, t, nt, left)) {
 #pragma unroll
       for (int e = 0; e < E; ++e) part[e] = mine[at(v, e, nt)];
     } else {
