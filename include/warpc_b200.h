@@ -219,6 +219,8 @@ const char* wg_kernel_name(int kernel_id);
  * Value types: WG_BF16, WG_FP16, WG_FP32.  Rows are `ld*` elements apart (>= the row's length); every ld is 64 bits.  No entry
  * synchronises or allocates but wg_int8_plan_create / _destroy / _last_device_status, so all of them may be captured into a
  * graph; calls on different streams share nothing but a plan's status words, which only a wait that gives up writes.
+ * Every launch of theirs may be set up while the launch before it in the stream ends; it reads and writes nothing before that one
+ * is complete, so stream order holds as for any launch.
  * Tokens, channels and a row's values: at most 2^30 each (WG_E_LIMIT). */
 enum { WG_BF16 = 0, WG_FP16 = 1, WG_FP32 = 2 };
 

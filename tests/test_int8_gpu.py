@@ -516,6 +516,44 @@ def test_a_block_in_8_bits(tokens, dtype):
     assert torch.equal(z, first)
 
 
+def test_order_of_launches_in_a_stream():
+    """Launches may be set up while the one before them ends: each step's buffers are rewritten by the next step without a
+    synchronisation between them, weights just before the product that reads them, and every step's result is kept."""
+    n, k, steps = 300, 700, 40
+    ld = up16(k)
+    g = gen(11)
+    for m in (1, 20, 90, 300):
+        xs = torch.randn(steps, m, k, generator=g, device="cuda").to(torch.bfloat16)
+        ws = torch.randn(steps, n, k, generator=g, device="cuda").to(torch.bfloat16)
+        wt = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+        x, r, qa, sa = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda"), torch.zeros(m, k, dtype=torch.bfloat16, device="cuda"), \
+            torch.zeros(m, ld, dtype=torch.int8, device="cuda"), torch.zeros(m, device="cuda")
+        b, qb, sb = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, ld, dtype=torch.int8, device="cuda"), torch.zeros(n, device="cuda")
+        y = torch.zeros(m, n, device="cuda")
+        plan = w.Int8Plan(n, k, qb.data_ptr(), sb.data_ptr(), out="fp32", ldb=ld)
+
+        def run(wait):
+            kept = []
+            r.zero_()
+            for i in range(steps):
+                x.copy_(xs[i])
+                b.copy_(ws[i])
+                w.quantise_rows(n, k, b.data_ptr(), qb.data_ptr(), sb.data_ptr(), ldq=ld)
+                wait()
+                w.norm_quantise_rows(m, k, x.data_ptr(), wt.data_ptr(), 1e-6, qa.data_ptr(), sa.data_ptr(), dR=r.data_ptr(), dH=r.data_ptr(), ldq=ld)
+                wait()
+                plan.launch(m, qa.data_ptr(), sa.data_ptr(), y.data_ptr(), lda=ld)
+                wait()
+                kept.append(y.clone())
+                plan.launch(m, qa.data_ptr(), sa.data_ptr(), y.data_ptr(), lda=ld)  # over what the copy reads
+            torch.cuda.synchronize()
+            return torch.stack(kept)
+
+        apart = run(torch.cuda.synchronize)
+        assert torch.equal(run(lambda: None), apart)
+        plan.status()
+
+
 @pytest.mark.parametrize("args", [["1", "300", "1111"], ["70", "260", "500", "2", "--norm"], ["300", "512", "640", "3", "--norm", "--out", "fp32"],
                                   ["5", "64", "64", "1", "--out", "fp16"]], ids=" ".join)
 def test_the_command(args, capsys):

@@ -20,6 +20,21 @@ bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t
 bool known_type(int dtype) { return dtype == WG_BF16 || dtype == WG_FP16 || dtype == WG_FP32; }
 int type_size(int dtype) { return dtype == WG_FP32 ? 4 : 2; }
 
+// One launch that may be set up while the one before it in the stream ends (the kernels wait for it before they touch global
+// memory); cluster: CTAs a cluster, 0 for a launch without clusters.
+int launch_kernel(const void* fn, dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, void** args) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster), attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = cluster > 0 ? 2 : 1;
+  return int(cudaLaunchKernelExC(&cfg, fn, args));
+}
+
 // ------------------------------------------------------------------ rows
 struct RowLaunch {
   int vpt, threads, rows, grid;
@@ -61,8 +76,8 @@ int launch_rows_shared(const RowParams& p, const RowLaunch& l, cudaStream_t stre
       raised.fetch_or(bit);
     }
   }
-  kernel<<<dim3(unsigned(l.grid)), dim3(unsigned(l.threads), unsigned(l.rows)), bytes, stream>>>(p);
-  return int(cudaGetLastError());
+  void* args[] = {const_cast<RowParams*>(&p)};
+  return launch_kernel((const void*)kernel, dim3(unsigned(l.grid)), dim3(unsigned(l.threads), unsigned(l.rows)), bytes, 0, stream, args);
 }
 
 template <class T, bool NORM, bool RES, bool VEC>
@@ -72,20 +87,14 @@ int launch_rows(RowParams p, cudaStream_t stream) {
   constexpr int NT = VEC ? 0 : 256;
   p.step = l.grid * l.rows;
   p.step_x = p.step * p.ldx, p.step_r = p.step * p.ldr, p.step_h = p.step * p.ldh, p.step_q = p.step * p.ldq;
-  if (!VEC && l.threads == 32) {
-    if (l.vpt == 1) rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 1, false><<<grid, block, 0, stream>>>(p);
-    else rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 2, false><<<grid, block, 0, stream>>>(p);
-  } else if (l.loop) {
-    rows_kernel<T, NORM, RES, VEC, NT, 4, true><<<grid, block, 0, stream>>>(p);
-  } else if (l.vpt == 1) {
-    rows_kernel<T, NORM, RES, VEC, NT, 1, false><<<grid, block, 0, stream>>>(p);
-  } else if (l.vpt == 2) {
-    if constexpr (VEC) return launch_rows_shared<T, NORM, RES>(p, l, stream);
-    else rows_kernel<T, NORM, RES, VEC, NT, 2, false><<<grid, block, 0, stream>>>(p);
-  } else if constexpr (!VEC) {
-    rows_kernel<T, NORM, RES, VEC, NT, 4, false><<<grid, block, 0, stream>>>(p);
-  }
-  return int(cudaGetLastError());
+  const void* kernel;
+  if (!VEC && l.threads == 32) kernel = l.vpt == 1 ? (const void*)rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 1, false> : (const void*)rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 2, false>;
+  else if (l.loop) kernel = (const void*)rows_kernel<T, NORM, RES, VEC, NT, 4, true>;
+  else if (l.vpt == 1) kernel = (const void*)rows_kernel<T, NORM, RES, VEC, NT, 1, false>;
+  else if constexpr (VEC) return launch_rows_shared<T, NORM, RES>(p, l, stream);
+  else kernel = l.vpt == 2 ? (const void*)rows_kernel<T, NORM, RES, VEC, NT, 2, false> : (const void*)rows_kernel<T, NORM, RES, VEC, NT, 4, false>;
+  void* args[] = {&p};
+  return launch_kernel(kernel, grid, block, 0, 0, stream, args);
 }
 
 template <class T, bool NORM, bool RES>
@@ -221,17 +230,8 @@ int i8_choose(int M, int N, int K, wg_int8_info* o) {
   return i8_derive(M, N, K, o);
 }
 
-template <class F>
-int launch(F* fn, const wg_int8_info& li, cudaStream_t stream, void** args) {
-  cudaLaunchConfig_t cfg;
-  std::memset(&cfg, 0, sizeof cfg);
-  cfg.gridDim = dim3(unsigned(li.grid)), cfg.blockDim = dim3(unsigned(li.threads));
-  cfg.dynamicSmemBytes = size_t(li.dynsmem), cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(li.cluster), attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr, cfg.numAttrs = li.cluster > 1 || li.kernel == WG_INT8_FEW ? 1 : 0;
-  return int(cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(fn), args));
+int launch(const void* fn, const wg_int8_info& li, cudaStream_t stream, void** args) {
+  return launch_kernel(fn, dim3(unsigned(li.grid)), dim3(unsigned(li.threads)), size_t(li.dynsmem), li.kernel == WG_INT8_GEMV ? 0 : li.cluster, stream, args);
 }
 
 // The kernels of one output type; `set_up` raises their shared-memory limit instead of launching.
@@ -248,19 +248,19 @@ struct I8Kernels {
     if (li.kernel == WG_INT8_GEMV) {
       void* args[] = {p};
       switch (li.tile_m) {
-        case 1: return launch(&i8_gemv_kernel<1, 4, OUT>, li, stream, args);
-        case 2: return launch(&i8_gemv_kernel<2, 4, OUT>, li, stream, args);
-        case 4: return launch(&i8_gemv_kernel<4, 4, OUT>, li, stream, args);
-        default: return launch(&i8_gemv_kernel<8, 4, OUT>, li, stream, args);
+        case 1: return launch((const void*)i8_gemv_kernel<1, 4, OUT>, li, stream, args);
+        case 2: return launch((const void*)i8_gemv_kernel<2, 4, OUT>, li, stream, args);
+        case 4: return launch((const void*)i8_gemv_kernel<4, 4, OUT>, li, stream, args);
+        default: return launch((const void*)i8_gemv_kernel<8, 4, OUT>, li, stream, args);
       }
     }
     if (li.kernel == WG_INT8_FEW) {
       void* args[] = {a, b, p};
-      return li.tile_m == 32 ? launch(&i8_few_kernel<FewCfg<32>, OUT>, li, stream, args) : launch(&i8_few_kernel<FewCfg<64>, OUT>, li, stream, args);
+      return li.tile_m == 32 ? launch((const void*)i8_few_kernel<FewCfg<32>, OUT>, li, stream, args) : launch((const void*)i8_few_kernel<FewCfg<64>, OUT>, li, stream, args);
     }
     void* args[] = {a, b, c, p};
-    if (li.tile_m == 256) return li.tile_n == 256 ? launch(&i8_tile_kernel<TileCfg<256, 256>, OUT>, li, stream, args) : launch(&i8_tile_kernel<TileCfg<256, 128>, OUT>, li, stream, args);
-    return li.tile_n == 128 ? launch(&i8_tile_kernel<TileCfg<128, 128>, OUT>, li, stream, args) : launch(&i8_tile_kernel<TileCfg<128, 64>, OUT>, li, stream, args);
+    if (li.tile_m == 256) return li.tile_n == 256 ? launch((const void*)i8_tile_kernel<TileCfg<256, 256>, OUT>, li, stream, args) : launch((const void*)i8_tile_kernel<TileCfg<256, 128>, OUT>, li, stream, args);
+    return li.tile_n == 128 ? launch((const void*)i8_tile_kernel<TileCfg<128, 128>, OUT>, li, stream, args) : launch((const void*)i8_tile_kernel<TileCfg<128, 64>, OUT>, li, stream, args);
   }
 };
 

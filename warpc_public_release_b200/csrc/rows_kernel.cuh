@@ -339,6 +339,9 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowPa
   constexpr int STAGES = kRowStages;
   extern __shared__ uint4 row_slots[];  // RING: [stage][v][thread]; SHARED_W: [v][thread]
   __shared__ float2 part[2][32];
+  // as the product's kernels: placed while the launch before ends, nothing read before it is complete
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int t = int(threadIdx.x), nt = NT ? NT : int(blockDim.x), lane = t & 31, warp = t >> 5, nw = nt >> 5;
   const int chunk = nt * VPT * E, left = p.K - S::first(t);
   const T* const w = static_cast<const T*>(p.w) + S::first(t);
