@@ -261,9 +261,11 @@ int wg_int8_launch(void* plan, int M, const signed char* dA, long long lda, cons
 /* Name the program of the launches that follow (kernel, tile_m, tile_n, split; the rest is derived), NULL: the rule's again.
  * WG_E_VARIANT where there is no such program; a launch with more tokens than a named gemv takes returns it too. */
 int wg_int8_plan_set_program(void* plan, const wg_int8_info* program);
-/* Bounded waits and their status, as wg_plan_set_timeout_ms and wg_last_device_status. */
+/* Bounded waits, their status and clearing it after a launch that gave up, as wg_plan_set_timeout_ms, wg_last_device_status and
+ * wg_plan_reset. */
 int wg_int8_plan_set_timeout_ms(void* plan, unsigned ms);
 int wg_int8_last_device_status(void* plan, unsigned out[4]);
+int wg_int8_plan_reset(void* plan);
 int wg_int8_plan_destroy(void* plan);
 
 const char* wg_strerror(int code);

@@ -67,6 +67,7 @@ def test_null_plans():
     assert l.wg_int8_plan_set_program(None, None) == WG_E_ARG
     assert l.wg_int8_plan_set_timeout_ms(None, 1) == WG_E_ARG
     assert l.wg_int8_last_device_status(None, None) == WG_E_ARG
+    assert l.wg_int8_plan_reset(None) == WG_E_ARG
     assert l.wg_int8_plan_destroy(None) == 0
     assert l.wg_int8_plan_create(0, 64, 64, P, 64, P, None, 0, None) == WG_E_ARG
 

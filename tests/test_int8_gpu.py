@@ -554,6 +554,38 @@ def test_order_of_launches_in_a_stream():
         plan.status()
 
 
+def test_first_calls_of_a_process_inside_a_capture():
+    """A process whose first launches are captured: nothing has to have run before (limits raised and code loaded in the capture)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, warpc_public_release_b200 as w
+m, k, n = 400, 8192, 256
+x = torch.randn(m, k, device="cuda").bfloat16(); f = torch.randn(m, k, device="cuda"); wt = torch.ones(k, device="cuda").bfloat16()
+q, q2, s = torch.zeros(m, k, dtype=torch.int8, device="cuda"), torch.zeros(m, k, dtype=torch.int8, device="cuda"), torch.zeros(m, device="cuda")
+s2, b, sb = torch.zeros(m, device="cuda"), torch.ones(n, k, dtype=torch.int8, device="cuda"), torch.ones(n, device="cuda")
+y, y1 = torch.zeros(m, n, device="cuda"), torch.zeros(3, n, device="cuda")
+plan = w.Int8Plan(n, k, b.data_ptr(), sb.data_ptr(), out="fp32")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    w.norm_quantise_rows(m, k, x.data_ptr(), wt.data_ptr(), 1e-6, q.data_ptr(), s.data_ptr(), stream=st)
+    w.quantise_rows(m, k, f.data_ptr(), q2.data_ptr(), s2.data_ptr(), dtype="fp32", stream=st)
+    plan.launch(m, q.data_ptr(), s.data_ptr(), y.data_ptr(), stream=st)
+    plan.launch(3, q2.data_ptr(), s2.data_ptr(), y1.data_ptr(), stream=st)
+g.replay(); torch.cuda.synchronize(); plan.status()
+assert torch.allclose(y, (q.double().sum(1) * s.double()).float()[:, None].expand(m, n), rtol=1e-6)
+assert torch.allclose(y1, (q2[:3].double().sum(1) * s2[:3].double()).float()[:, None].expand(3, n), rtol=1e-6)
+plan.reset()
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=200)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
 @pytest.mark.parametrize("args", [["1", "300", "1111"], ["70", "260", "500", "2", "--norm"], ["300", "512", "640", "3", "--norm", "--out", "fp32"],
                                   ["5", "64", "64", "1", "--out", "fp16"]], ids=" ".join)
 def test_the_command(args, capsys):

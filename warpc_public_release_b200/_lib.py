@@ -99,6 +99,7 @@ def lib():
         "wg_int8_plan_set_timeout_ms": ([vp, u], i),
         "wg_int8_launch": ([vp, i, vp, ll, vp, vp, ll, vp], i),
         "wg_int8_last_device_status": ([vp, ctypes.POINTER(u * 4)], i),
+        "wg_int8_plan_reset": ([vp], i),
         "wg_int8_plan_destroy": ([vp], i),
         "wg_kernel_count": ([], i),
         "wg_kernel_name": ([i], ctypes.c_char_p),

@@ -401,6 +401,15 @@ extern "C" int wg_int8_last_device_status(void* plan, unsigned out[4]) {
   return out[0] == 0 ? WG_OK : WG_E_DEVICE_WAIT;
 }
 
+extern "C" int wg_int8_plan_reset(void* plan) {
+  I8Plan* pl = static_cast<I8Plan*>(plan);
+  if (!pl) return WG_E_ARG;
+  WG_ON_DEVICE(pl->device);
+  WG_CUDA(cudaDeviceSynchronize());
+  WG_CUDA(cudaMemset(pl->d_status, 0, 4 * sizeof(uint32_t)));
+  return WG_OK;
+}
+
 extern "C" int wg_int8_plan_destroy(void* plan) {
   I8Plan* pl = static_cast<I8Plan*>(plan);
   if (!pl) return WG_OK;

@@ -78,6 +78,9 @@ class Int8Plan:
         check(r, "wg_int8_last_device_status")
         return tuple(st)
 
+    def reset(self):
+        check(_lib.lib().wg_int8_plan_reset(self._h), "wg_int8_plan_reset")
+
     def close(self):
         if self._h is not None:
             _lib.lib().wg_int8_plan_destroy(self._h)
