@@ -93,10 +93,13 @@ def test_every_program_at_ragged_sizes(program, shape):
 @pytest.mark.parametrize("out", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("program", [("gemv", 2, 0, 2), ("few", 32, 128, 4), ("tile", 256, 256, 1), ("tile", 256, 128, 1), ("tile", 128, 128, 1), ("tile", 128, 64, 1)],
                          ids=lambda p: "-".join(map(str, p)))
-@pytest.mark.parametrize("layout", ["aligned", "wide", "odd stride", "odd start"])
+@pytest.mark.parametrize("layout", ["aligned", "wide", "stride of 8 bytes", "stride of 4 bytes", "odd stride", "odd start", "odd length"])
 def test_output_types_and_layouts(out, program, layout):
     m, n, k = (2 if program[0] == "gemv" else 290), 328, 640
-    ldc, shift = {"aligned": (n, 0), "wide": (n + 24, 0), "odd stride": (n + 1, 0), "odd start": (n, 1)}[layout]
+    step = 1 if out == "fp32" else 2
+    n = n - 3 if layout == "odd length" else n  # rows in pieces of 8 bytes, the last piece cut
+    ldc, shift = {"aligned": (n, 0), "wide": (n + 24, 0), "stride of 8 bytes": (n + 2 * step, 0), "stride of 4 bytes": (n + step, 0), "odd stride": (n + 1, 0),
+                  "odd start": (n, 1), "odd length": (n + 3 + 2 * step, 2 * step)}[layout]
     run_product(m, n, k, out, bias=True, program=program, ldc=ldc, shift=shift, lda=k + 48, ldb=k + 16)
 
 
@@ -298,7 +301,8 @@ def test_quantise_lengths(dtype, k):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("ld,shift,ldq,qshift", [(1111, 0, 1120, 0), (1112, 0, 1111, 3), (1200, 8, 1112, 0), (1200, 1, 1112, 8), (1201, 0, 1136, 4), (1104, 0, 1104, 0)])
+@pytest.mark.parametrize("ld,shift,ldq,qshift", [(1111, 0, 1120, 0), (1112, 0, 1111, 3), (1200, 8, 1112, 0), (1200, 1, 1112, 8), (1201, 0, 1136, 4), (1204, 0, 1112, 0), (1204, 4, 1120, 4),
+                                                  (1202, 2, 1116, 2), (1104, 0, 1104, 0)])
 def test_quantise_strides_and_alignment(dtype, ld, shift, ldq, qshift):
     x = rows_of(40, 1104 if ld == 1104 else 1111, dtype, 5, ld, shift)
     q, scale = run_quantise(x, dtype, ldq, qshift)
@@ -397,7 +401,7 @@ def test_norm_lengths(dtype, residual, k):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("ld,shift", [(1111, 0), (1200, 0), (1200, 1), (1201, 8)])
+@pytest.mark.parametrize("ld,shift", [(1111, 0), (1200, 0), (1200, 1), (1201, 8), (1204, 0), (1202, 2)])
 def test_norm_strides_and_in_place(dtype, ld, shift):
     """Any stride and start; the sum in its own memory, in the residual's, in x's."""
     k = 1111
@@ -408,6 +412,23 @@ def test_norm_strides_and_in_place(dtype, ld, shift):
         q, scale, h = run_norm(x, r, wt, dtype, h={"own": None, "x": x, "r": r}[where])
         assert torch.equal(q, want) and torch.equal(h, h64)
         assert bool(((scale.double() - s).abs() <= scale_tolerance(k) * s).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("k", [70, 500, 1029, 2500, 4100, 6003, 8204, 12001, 16390, 33001])
+def test_norm_rows_of_every_alignment(dtype, k):
+    """Every width of access with every way a row is spread over threads: rows 16, 8, 4 and 2 bytes apart from a boundary."""
+    wt = (1 + 0.3 * torch.randn(k, generator=gen(9), device="cuda")).to(TYPES[dtype])
+    for m in (5, 400):
+        for extra in (0, 1, 2, 4, 8):
+            ld = -(-k // 8) * 8 + extra
+            x, r = rows_of(m, k, dtype, 1, ld), rows_of(m, k, dtype, 2, ld)
+            h = torch.empty(m, ld, dtype=TYPES[dtype], device="cuda")[:, :k]
+            for residual in (None, r):
+                want, s, h64 = norm64(x, residual, wt, 1e-6)
+                q, scale, got = run_norm(x, residual, wt, dtype, h=h if residual is not None else None)
+                assert torch.equal(q, want) and (residual is None or torch.equal(got, h64))
+                assert bool(((scale.double() - s).abs() <= scale_tolerance(k) * s).all())
 
 
 @pytest.mark.parametrize("k", [40, 1111, 5000, 40000])

@@ -41,20 +41,21 @@ struct RowLaunch {
   bool loop;
 };
 
-// How a row is spread: `slots` vectors of 16 bytes.  A warp a row up to 64 vectors (no barrier); else a block a row, one
-// vector a thread where there are too few rows to fill the machine and only a row's own latency counts, two otherwise.
-RowLaunch row_launch(int M, int slots, bool vec) {
+// How a row is spread: `slots` vectors of 16 bytes.  A warp a row up to 64 of them (no barrier); else a block a row.  Rows of
+// 16-byte accesses: one slot a thread where there are too few rows to fill the machine and only a row's own latency counts, two
+// otherwise.  Rows of narrower accesses: 256 threads with one or two slots, then 512 or 1024 with two.  Rows beyond 2048 slots are
+// read twice.
+RowLaunch row_launch(int M, int slots, bool wide) {
   RowLaunch l;
-  l.loop = false;
+  l.loop = slots > 2048, l.rows = 1;
   if (slots <= 64) {
-    l.vpt = slots <= 32 ? 1 : 2, l.threads = 32, l.rows = M > 4 * kSms ? 8 : 1;
+    l.vpt = wide && slots <= 32 ? 1 : 2, l.threads = 32, l.rows = M > 4 * kSms ? 8 : 1;
+  } else if (wide) {
+    l.vpt = l.loop ? 4 : slots <= 1024 && M <= 2 * kSms ? 1 : 2;
+    l.threads = l.loop ? 512 : (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32;
   } else {
-    l.rows = 1;
-    // vectors: up to 1024 threads with two each; scalar rows: 256 threads with one, two or four slots each
-    const int block = vec ? 1024 : 256;
-    l.vpt = slots <= block && (M <= 2 * kSms || !vec) ? 1 : slots <= 2 * block ? 2 : 4;
-    l.loop = slots > (vec ? 2 : 4) * block;
-    l.threads = !vec ? 256 : l.loop ? 512 : (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32;
+    l.vpt = slots <= 256 ? 1 : 2;
+    l.threads = l.loop ? 512 : slots <= 512 ? 256 : slots <= 1024 ? 512 : 1024;
   }
   const int per_sm = std::max(1, (l.vpt <= 2 ? 1024 : 512) / (l.threads * l.rows));
   l.grid = int(std::min(((long long)M + l.rows - 1) / l.rows, (long long)kSms * per_sm));
@@ -65,7 +66,7 @@ RowLaunch row_launch(int M, int slots, bool vec) {
 template <class T, bool NORM, bool RES>
 int launch_rows_shared(const RowParams& p, const RowLaunch& l, cudaStream_t stream) {
   static std::atomic<unsigned long long> raised{0};
-  const auto kernel = &rows_kernel<T, NORM, RES, true, 0, 2, false>;
+  const auto kernel = &rows_kernel<T, NORM, RES, 16, 0, 2, false>;
   const size_t bytes = size_t(l.threads) * l.rows * kRowWords<NORM> * 16;
   if (bytes > 32 * 1024) {  // with the kernel's own words, 48 KB need no asking
     int device = 0;
@@ -80,31 +81,41 @@ int launch_rows_shared(const RowParams& p, const RowLaunch& l, cudaStream_t stre
   return launch_kernel((const void*)kernel, dim3(unsigned(l.grid)), dim3(unsigned(l.threads), unsigned(l.rows)), bytes, 0, stream, args);
 }
 
-template <class T, bool NORM, bool RES, bool VEC>
+template <class T, bool NORM, bool RES, int W>
 int launch_rows(RowParams p, cudaStream_t stream) {
-  const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E, VEC);
-  const dim3 block(unsigned(l.threads), unsigned(l.rows)), grid(unsigned(l.grid));
-  constexpr int NT = VEC ? 0 : 256;
+  const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E, W == 16);
   p.step = l.grid * l.rows;
   p.step_x = p.step * p.ldx, p.step_r = p.step * p.ldr, p.step_h = p.step * p.ldh, p.step_q = p.step * p.ldq;
   const void* kernel;
-  if (!VEC && l.threads == 32) kernel = l.vpt == 1 ? (const void*)rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 1, false> : (const void*)rows_kernel<T, NORM, RES, VEC, VEC ? 0 : 32, 2, false>;
-  else if (l.loop) kernel = (const void*)rows_kernel<T, NORM, RES, VEC, NT, 4, true>;
-  else if (l.vpt == 1) kernel = (const void*)rows_kernel<T, NORM, RES, VEC, NT, 1, false>;
-  else if constexpr (VEC) return launch_rows_shared<T, NORM, RES>(p, l, stream);
-  else kernel = l.vpt == 2 ? (const void*)rows_kernel<T, NORM, RES, VEC, NT, 2, false> : (const void*)rows_kernel<T, NORM, RES, VEC, NT, 4, false>;
+  if constexpr (W == 16) {
+    if (l.vpt == 2) return launch_rows_shared<T, NORM, RES>(p, l, stream);
+    kernel = l.loop ? (const void*)rows_kernel<T, NORM, RES, W, 0, 4, true> : (const void*)rows_kernel<T, NORM, RES, W, 0, 1, false>;
+  } else if (l.loop) {
+    kernel = (const void*)rows_kernel<T, NORM, RES, W, 512, 2, true>;
+  } else {
+    kernel = l.threads == 32 ? (const void*)rows_kernel<T, NORM, RES, W, 32, 2, false>
+             : l.vpt == 1    ? (const void*)rows_kernel<T, NORM, RES, W, 256, 1, false>
+             : l.threads == 256 ? (const void*)rows_kernel<T, NORM, RES, W, 256, 2, false>
+             : l.threads == 512 ? (const void*)rows_kernel<T, NORM, RES, W, 512, 2, false>
+                                : (const void*)rows_kernel<T, NORM, RES, W, 1024, 2, false>;
+  }
   void* args[] = {&p};
-  return launch_kernel(kernel, grid, block, 0, 0, stream, args);
+  return launch_kernel(kernel, dim3(unsigned(l.grid)), dim3(unsigned(l.threads), unsigned(l.rows)), 0, 0, stream, args);
 }
 
+// The widest access that every row of every operand is aligned to.
 template <class T, bool NORM, bool RES>
 int launch_rows_as(const RowParams& p, cudaStream_t stream) {
-  const unsigned bytes = 16, qbytes = RowVec<T>::E;
-  auto whole = [&](long long ld, unsigned size) { return p.M == 1 || (ld * size) % bytes == 0; };
-  bool vec = aligned(p.x, bytes) && whole(p.ldx, sizeof(T)) && aligned(p.q, qbytes) && (p.M == 1 || p.ldq % qbytes == 0);
-  if (NORM) vec = vec && aligned(p.w, bytes);
-  if (RES) vec = vec && aligned(p.r, bytes) && aligned(p.h, bytes) && whole(p.ldr, sizeof(T)) && whole(p.ldh, sizeof(T));
-  return vec ? launch_rows<T, NORM, RES, true>(p, stream) : launch_rows<T, NORM, RES, false>(p, stream);
+  auto fits = [&](unsigned width) {
+    auto rows = [&](const void* at, long long ld) { return aligned(at, width) && (p.M == 1 || (ld * int(sizeof(T))) % width == 0); };
+    const unsigned bytes = width / unsigned(sizeof(T));  // of q
+    return rows(p.x, p.ldx) && aligned(p.q, bytes) && (p.M == 1 || p.ldq % bytes == 0) && (!NORM || aligned(p.w, width)) &&
+           (!RES || (rows(p.r, p.ldr) && rows(p.h, p.ldh)));
+  };
+  if (fits(16)) return launch_rows<T, NORM, RES, 16>(p, stream);
+  if (fits(8)) return launch_rows<T, NORM, RES, 8>(p, stream);
+  if (sizeof(T) == 4 || fits(4)) return launch_rows<T, NORM, RES, 4>(p, stream);
+  return launch_rows<T, NORM, RES, sizeof(T) == 4 ? 4 : 2>(p, stream);
 }
 
 template <bool NORM, bool RES>
@@ -373,14 +384,14 @@ extern "C" int wg_int8_launch(void* plan, int M, const signed char* dA, long lon
   p.depth = li.depth, p.group = 8, p.wk = li.split;
   p.A = reinterpret_cast<const int8_t*>(dA), p.Bt = pl->Bt, p.lda = lda, p.ldb = pl->ldb, p.ldc = ldc;
   p.sa = dScaleA, p.sb = pl->sb, p.bias = pl->bias, p.C = dC, p.status = pl->d_status, p.timeout_ns = pl->timeout_ns;
-  p.tma_store = aligned(dC, 16) && (ldc * size) % 16 == 0;
+  for (p.store_bytes = 16; p.store_bytes > size && !(aligned(dC, unsigned(p.store_bytes)) && (ldc * size) % p.store_bytes == 0);) p.store_bytes /= 2;
   WG_ON_DEVICE(pl->device);
   CUtensorMap map_a, map_c;
   std::memset(&map_a, 0, sizeof map_a), std::memset(&map_c, 0, sizeof map_c);
   CUtensorMap* map_b = li.kernel == WG_INT8_TILE && li.tile_n / li.cluster == 64 ? &pl->map_b64 : &pl->map_b128;
   if (li.kernel != WG_INT8_GEMV)
     if ((r = encode_rows(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dA, M, pl->K, lda, li.kernel == WG_INT8_FEW ? li.tile_m : 128)) != WG_OK) return r;
-  if (li.kernel == WG_INT8_TILE && p.tma_store) {
+  if (li.kernel == WG_INT8_TILE && p.store_bytes == 16) {
     const CUtensorMapDataType type = pl->out == WG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : pl->out == WG_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     if ((r = encode_rows(&map_c, type, size, dC, M, pl->N, ldc, 32)) != WG_OK) return r;
   }

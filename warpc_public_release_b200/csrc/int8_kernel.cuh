@@ -36,7 +36,7 @@ struct I8Params {
   int tiles_m, tiles_n;  // tiles of tokens and of channels
   int depth;             // ring rounds (of KSUB k-steps)
   int group;             // tile rows walked down before moving across
-  int tma_store;         // Y's rows are 16-byte aligned: whole boxes go out through the copy engine
+  int store_bytes;       // what Y's rows are aligned to: 16 (whole boxes go out through the copy engine), 8, 4 or 2
   int wk;                // gemv: warps that share a channel's K
   const int8_t* A;       // gemv reads plain memory
   const int8_t* Bt;
@@ -240,6 +240,46 @@ WB_DEV void i8_channel(const float* src, int n, int N, float* out) {
   }
 }
 
+// A staged copy (32 rows of 128 bytes, swizzled) to rows of Y aligned to U bytes only: U bytes a lane, neighbouring lanes
+// neighbouring memory, as many rows at a time as that leaves lanes for.
+template <class T, int U>
+WB_DEV void i8_store_rows(uint32_t copy, T* out, int m0, int M, int n0, int N, long long ldc, uint32_t lane) {
+  constexpr int LANES = 128 / U < 32 ? 128 / U : 32, ROWS = 32 / LANES, E = U / int(sizeof(T));
+#pragma unroll 4
+  for (uint32_t i = 0; i < 32; i += ROWS) {
+    const uint32_t row = i + lane / LANES;
+#pragma unroll
+    for (uint32_t byte = (lane % LANES) * U; byte < 128; byte += LANES * U) {
+      const uint32_t at = copy + row * 128u + (((byte >> 4) ^ (row & 7u)) << 4) + (byte & 15u);
+      const int n = n0 + int(byte) / int(sizeof(T));
+      if (m0 + int(row) >= M || n >= N) continue;
+      T* const to = out + (long long)(m0 + int(row)) * ldc + n;
+      T v[E];
+      if constexpr (U == 8) {
+        uint2 w;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(at) : "memory");
+        memcpy(v, &w, 8);
+        if (n + E <= N) *reinterpret_cast<uint2*>(to) = w;
+      } else if constexpr (U == 4) {
+        uint32_t w;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+        memcpy(v, &w, 4);
+        if (n + E <= N) *reinterpret_cast<uint32_t*>(to) = w;
+      } else {
+        uint16_t w;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at) : "memory");
+        memcpy(v, &w, 2);
+        *reinterpret_cast<uint16_t*>(to) = w;
+      }
+      if (E > 1 && n + E > N) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (n + e < N) to[e] = v[e];
+      }
+    }
+  }
+}
+
 template <class C, int OUT>
 __global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                          const __grid_constant__ CUtensorMap map_c, const __grid_constant__ I8Params p) {
@@ -369,34 +409,18 @@ __global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(con
         }
         if (OUT != I8_FP32 && half == 0) continue;
         const int nc = n0 + (OUT == I8_FP32 ? 32 * b : 32 * (b - half));
-        if (p.tma_store) {
+        if (p.store_bytes == 16) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
             if (m0 < p.M && nc < p.N) tma_store_2d(&map_c, nc, m0, copy);
             bulk_commit();
           }
-        } else {  // rows of Y that the copy engine cannot write: a row at a time, neighbouring lanes neighbouring channels
+        } else {  // rows of Y that the copy engine cannot write
           __syncwarp();
-          for (int i = 0; i < 32 && m0 + i < p.M; ++i) {
-#pragma unroll
-            for (int j = 0; j < L::WIDTH; j += 32) {
-              const uint32_t byte = (uint32_t(j) + lane) * uint32_t(sizeof(T));
-              const uint32_t at = copy + uint32_t(i) * 128u + (((byte >> 4) ^ (uint32_t(i) & 7u)) << 4) + (byte & 15u);
-              if (nc + j + int(lane) < p.N) {
-                T* const to = out + (long long)(m0 + i) * p.ldc + nc + j + int(lane);
-                if constexpr (OUT == I8_FP32) {
-                  uint32_t w;
-                  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
-                  *reinterpret_cast<uint32_t*>(to) = w;
-                } else {
-                  uint16_t w;
-                  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at) : "memory");
-                  *reinterpret_cast<uint16_t*>(to) = w;
-                }
-              }
-            }
-          }
+          if (p.store_bytes == 8) i8_store_rows<T, 8>(copy, out, m0, p.M, nc, p.N, p.ldc, lane);
+          else if (sizeof(T) == 4 || p.store_bytes == 4) i8_store_rows<T, 4>(copy, out, m0, p.M, nc, p.N, p.ldc, lane);
+          else i8_store_rows<T, sizeof(T) == 4 ? 4 : 2>(copy, out, m0, p.M, nc, p.N, p.ldc, lane);
           __syncwarp();
         }
       }
@@ -534,7 +558,7 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] = p.bias != nullptr ? i8_value(sum[j], sa, sb[j], add[j]) : i8_value(sum[j], sa, sb[j]);
       T* const to = out + (long long)m * p.ldc + n;
-      if (p.tma_store && n + 4 <= p.N) {  // Y's rows are 16-byte aligned
+      if (p.store_bytes >= 4 * int(sizeof(T)) && n + 4 <= p.N) {
         if constexpr (OUT == I8_FP32) *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
         else *reinterpret_cast<uint2*>(to) = make_uint2(I8Out<OUT>::two(y[0], y[1]), I8Out<OUT>::two(y[2], y[3]));
       } else {

@@ -148,64 +148,84 @@ struct RowVec<float> {
   }
 };
 
-// Where a thread's values sit in its row: slot v (of E values) of NT threads' slots side by side.  VEC: one 16-byte vector; else
-// values `nt` apart, so that the lanes of a warp read neighbouring values whatever the rows' alignment.  `mine` points at the
-// thread's first value, `left` values of the row lie from there on (the row's own, not the thread's: the thread has every E-th
-// vector, or every nt-th value, of them).
-template <class T, bool VEC>
+// Where a thread's values sit in its row.  Memory is accessed W bytes at a time, as wide as the rows' alignment allows; a slot is 16
+// bytes of a thread, 16 / W accesses that lie `nt` threads' accesses apart, so that the lanes of a warp always touch neighbouring
+// memory.  `mine` points at the thread's first value, `left` is how many values of the row lie from there to its end.
+template <class T, int W>
 struct RowSlot {
   using V = RowVec<T>;
-  static constexpr int E = V::E;
-  static __device__ __forceinline__ int first(int t) { return VEC ? t * E : t; }
-  static __device__ __forceinline__ int at(int v, int e, int nt) { return VEC ? v * nt * E + e : (v * E + e) * nt; }
-  // all E values exist; scalar rows ask for all threads at once (the thread nt - 1 places on has the fewest left)
-  static __device__ __forceinline__ bool whole(int v, int t, int nt, int left) { return VEC ? at(v, E - 1, nt) < left : (v + 1) * E * nt - t <= left; }
+  static constexpr int E = V::E, EW = W / int(sizeof(T)), S = 16 / W;
+  static __device__ __forceinline__ int first(int t) { return t * EW; }
+  static __device__ __forceinline__ int at(int v, int e, int nt) { return (v * S + e / EW) * nt * EW + e % EW; }
+  // all E values exist; with several accesses a slot asked for all threads at once (the last thread has the fewest left)
+  static __device__ __forceinline__ bool whole(int v, int t, int nt, int left) { return S == 1 ? at(v, E - 1, nt) < left : (v + 1) * S * nt * EW - first(t) <= left; }
+
+  // access j of slot v: does it lie inside the row / does any of it
+  static __device__ __forceinline__ bool inside(int v, int j, int nt, int left) { return at(v, j * EW + EW - 1, nt) < left; }
+  static __device__ __forceinline__ bool touches(int v, int j, int nt, int left) { return EW > 1 && at(v, j * EW, nt) < left; }
 
   static __device__ __forceinline__ uint4 load(const T* mine, int v, int t, int nt, int left) {
-    if constexpr (VEC) {
-      if (whole(v, t, nt, left)) return *reinterpret_cast<const uint4*>(mine + at(v, 0, nt));
+    if constexpr (W == 16) {
+      if (inside(v, 0, nt, left)) return *reinterpret_cast<const uint4*>(mine + at(v, 0, nt));
     }
-    T part[E];
-    if (!VEC && whole(v, t, nt, left)) {
+    uint32_t u[4] = {0u, 0u, 0u, 0u};
+    const bool all = W != 16 && whole(v, t, nt, left);
 #pragma unroll
-      for (int e = 0; e < E; ++e) part[e] = mine[at(v, e, nt)];
-    } else {
+    for (int j = 0; j < S; ++j) {
+      const T* const from = mine + at(v, j * EW, nt);
+      if (W != 16 && (all || inside(v, j, nt, left))) {
+        if constexpr (W == 8) {
+          const uint2 d = *reinterpret_cast<const uint2*>(from);
+          u[(2 * j) % 4] = d.x, u[(2 * j + 1) % 4] = d.y;
+        } else if constexpr (W == 4) {
+          u[j] = *reinterpret_cast<const uint32_t*>(from);
+        } else if constexpr (W == 2) {
+          u[j / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(from)) << (16 * (j % 2));
+        }
+      } else if (touches(v, j, nt, left)) {  // the row ends inside
+        T part[EW];
 #pragma unroll
-      for (int e = 0; e < E; ++e) part[e] = at(v, e, nt) < left ? mine[at(v, e, nt)] : T(0.0f);
-    }
-    uint4 u;
-    memcpy(&u, part, 16);
-    return u;
-  }
-  static __device__ __forceinline__ void store(T* mine, const uint4& u, int v, int t, int nt, int left) {
-    T part[E];
-    memcpy(part, &u, 16);
-    if (whole(v, t, nt, left)) {
-      if constexpr (VEC) {
-        *reinterpret_cast<uint4*>(mine + at(v, 0, nt)) = u;
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) mine[at(v, e, nt)] = part[e];
+        for (int e = 0; e < EW; ++e) part[e] = at(v, j * EW + e, nt) < left ? from[e] : T(0.0f);
+        memcpy(reinterpret_cast<char*>(u) + j * W, part, W);
       }
-    } else {
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ void store(T* mine, const uint4& w, int v, int t, int nt, int left) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    const bool all = whole(v, t, nt, left);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (at(v, e, nt) < left) mine[at(v, e, nt)] = part[e];
+    for (int j = 0; j < S; ++j) {
+      T* const to = mine + at(v, j * EW, nt);
+      if (all || inside(v, j, nt, left)) {
+        if constexpr (W == 16) *reinterpret_cast<uint4*>(to) = w;
+        else if constexpr (W == 8) *reinterpret_cast<uint2*>(to) = make_uint2(u[(2 * j) % 4], u[(2 * j + 1) % 4]);
+        else if constexpr (W == 4) *reinterpret_cast<uint32_t*>(to) = u[j];
+        else *reinterpret_cast<uint16_t*>(to) = uint16_t(u[j / 2] >> (16 * (j % 2)));
+      } else if (touches(v, j, nt, left)) {
+        T part[EW];
+        memcpy(part, reinterpret_cast<const char*>(u) + j * W, W);
+#pragma unroll
+        for (int e = 0; e < EW; ++e)
+          if (at(v, j * EW + e, nt) < left) to[e] = part[e];
+      }
     }
   }
   static __device__ __forceinline__ void store_q(int8_t* mine, const uint32_t* q4, int v, int t, int nt, int left) {
-    if (whole(v, t, nt, left)) {
-      if constexpr (VEC) {
-        if constexpr (E == 8) *reinterpret_cast<uint2*>(mine + at(v, 0, nt)) = make_uint2(q4[0], q4[1]);
-        else *reinterpret_cast<uint32_t*>(mine + at(v, 0, nt)) = q4[0];
-      } else {
+    const bool all = whole(v, t, nt, left);
 #pragma unroll
-        for (int e = 0; e < E; ++e) mine[at(v, e, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
+    for (int j = 0; j < S; ++j) {
+      int8_t* const to = mine + at(v, j * EW, nt);
+      if (all || inside(v, j, nt, left)) {
+        if constexpr (EW == 8) *reinterpret_cast<uint2*>(to) = make_uint2(q4[0], q4[1]);
+        else if constexpr (EW == 4) *reinterpret_cast<uint32_t*>(to) = q4[j];
+        else if constexpr (EW == 2) *reinterpret_cast<uint16_t*>(to) = uint16_t(q4[j / 2] >> (16 * (j % 2)));
+        else *to = int8_t(q4[j / 4] >> (8 * (j % 4)));
+      } else if (touches(v, j, nt, left)) {
+#pragma unroll
+        for (int e = 0; e < EW; ++e)
+          if (at(v, j * EW + e, nt) < left) to[e] = int8_t(q4[(j * EW + e) / 4] >> (8 * ((j * EW + e) % 4)));
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (at(v, e, nt) < left) mine[at(v, e, nt)] = int8_t(q4[e / 4] >> (8 * (e % 4)));
     }
   }
 };
@@ -313,7 +333,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 
 // blockDim = (threads a row, rows a block): more than 32 threads a row only with one row a block.  NT: the threads a row where
-// they are known (scalar rows: their addresses become constants), else 0.  VPT vectors of 16 bytes a thread; LOOP: rows longer
+// they are known (rows of narrow accesses: their addresses become constants), else 0.  VPT vectors of 16 bytes a thread; LOOP: rows longer
 // than a block holds, read a second time (from L2) for the second half of the work.
 // RING: rows of vectors that are only quantised have the loads of the next three rows out while one is reduced and written, in
 // slots of shared memory that only the thread itself reads (so nothing but its own copies is waited for): with the next row in
@@ -322,20 +342,20 @@ __device__ __forceinline__ double warp_sum(double v) {
 // short there is instructions and registers.  SHARED_W: the norm's weights, the same for all of a block's rows, in such slots too:
 // two loads a row instead of eight registers held (49 -> 45.1, fp32 71.9 -> 69.3, 40.9 -> 34.4 without a residual).
 constexpr int kRowStages = 4;
-template <bool NORM, bool VEC, int VPT, bool LOOP>
-constexpr bool kRowRing = !NORM && VEC && VPT == 2 && !LOOP;
-template <bool NORM, bool VEC, int VPT, bool LOOP>
-constexpr bool kRowSharedW = NORM && VEC && VPT == 2 && !LOOP;
+template <bool NORM, int W, int VPT, bool LOOP>
+constexpr bool kRowRing = !NORM && W == 16 && VPT == 2 && !LOOP;
+template <bool NORM, int W, int VPT, bool LOOP>
+constexpr bool kRowSharedW = NORM && W == 16 && VPT == 2 && !LOOP;
 template <bool NORM>  // 16-byte words of shared memory a thread of these kernels
 constexpr int kRowWords = 2 * (NORM ? 1 : kRowStages);
 
-template <class T, bool NORM, bool RES, bool VEC, int NT, int VPT, bool LOOP>
+template <class T, bool NORM, bool RES, int W, int NT, int VPT, bool LOOP>
 __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowParams p) {
   static_assert(NORM || !RES, "the residual comes with the norm");
-  using S = RowSlot<T, VEC>;
+  using S = RowSlot<T, W>;
   using V = typename S::V;
   constexpr int E = S::E, P = E / 2;
-  constexpr bool SHORT = !NORM && sizeof(T) == 2, RING = kRowRing<NORM, VEC, VPT, LOOP>, SHARED_W = kRowSharedW<NORM, VEC, VPT, LOOP>;
+  constexpr bool SHORT = !NORM && sizeof(T) == 2, RING = kRowRing<NORM, W, VPT, LOOP>, SHARED_W = kRowSharedW<NORM, W, VPT, LOOP>;
   constexpr int STAGES = kRowStages;
   extern __shared__ uint4 row_slots[];  // RING: [stage][v][thread]; SHARED_W: [v][thread]
   __shared__ float2 part[2][32];
