@@ -41,24 +41,27 @@ struct RowLaunch {
   bool loop;
 };
 
-// How a row is spread: `slots` vectors of 16 bytes.  A warp a row up to 64 of them (no barrier); else a block a row.  Rows of
-// 16-byte accesses: one slot a thread where there are too few rows to fill the machine and only a row's own latency counts, two
-// otherwise.  Rows of narrower accesses: 256 threads with one or two slots, then 512 or 1024 with two.  Rows beyond 2048 slots are
-// read twice.
+// How a row is spread: `slots` vectors of 16 bytes.  A warp a row up to 64 of them (no barrier); else a block a row.  Rows of 16-
+// or 8-byte accesses: one slot a thread where there are too few rows to fill the machine and only a row's own latency counts, two
+// otherwise, and as many threads as that takes.  Rows of 4- or 2-byte accesses: 256 threads with one or two slots, then 512 or
+// 1024 with two, as constants (a slot is four or eight accesses, whose addresses are constants then: 16384 x 4095 bf16 with a
+// residual 232 -> 138-148 us; with 8-byte accesses the slots that stay empty cost more: 1792 x 4516 fp16 16.9 against 30.5).
+// Rows beyond 2048 slots are read twice.
 RowLaunch row_launch(int M, int slots, bool wide) {
   RowLaunch l;
   l.loop = slots > 2048, l.rows = 1;
   if (slots <= 64) {
-    l.vpt = wide && slots <= 32 ? 1 : 2, l.threads = 32, l.rows = M > 4 * kSms ? 8 : 1;
+    l.vpt = slots <= 32 ? 1 : 2, l.threads = 32, l.rows = M > 4 * kSms ? 8 : 1;
+  } else if (l.loop) {
+    l.vpt = wide ? 4 : 2, l.threads = 512;
   } else if (wide) {
-    l.vpt = l.loop ? 4 : slots <= 1024 && M <= 2 * kSms ? 1 : 2;
-    l.threads = l.loop ? 512 : (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32;
+    l.vpt = slots <= 1024 && M <= 2 * kSms ? 1 : 2;
+    l.threads = (((slots + l.vpt - 1) / l.vpt) + 31) / 32 * 32;
   } else {
     l.vpt = slots <= 256 ? 1 : 2;
-    l.threads = l.loop ? 512 : slots <= 512 ? 256 : slots <= 1024 ? 512 : 1024;
+    l.threads = slots <= 512 ? 256 : slots <= 1024 ? 512 : 1024;
   }
-  const int per_sm = std::max(1, (l.vpt <= 2 ? 1024 : 512) / (l.threads * l.rows));
-  l.grid = int(std::min(((long long)M + l.rows - 1) / l.rows, (long long)kSms * per_sm));
+  l.grid = int(std::min(((long long)M + l.rows - 1) / l.rows, (long long)kSms * std::max(1, 1024 / (l.threads * l.rows))));
   return l;
 }
 
@@ -83,21 +86,20 @@ int launch_rows_shared(const RowParams& p, const RowLaunch& l, cudaStream_t stre
 
 template <class T, bool NORM, bool RES, int W>
 int launch_rows(RowParams p, cudaStream_t stream) {
-  const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E, W == 16);
+  const RowLaunch l = row_launch(p.M, (p.K + RowVec<T>::E - 1) / RowVec<T>::E, W >= 8);
   p.step = l.grid * l.rows;
   p.step_x = p.step * p.ldx, p.step_r = p.step * p.ldr, p.step_h = p.step * p.ldh, p.step_q = p.step * p.ldq;
   const void* kernel;
-  if constexpr (W == 16) {
-    if (l.vpt == 2) return launch_rows_shared<T, NORM, RES>(p, l, stream);
-    kernel = l.loop ? (const void*)rows_kernel<T, NORM, RES, W, 0, 4, true> : (const void*)rows_kernel<T, NORM, RES, W, 0, 1, false>;
-  } else if (l.loop) {
-    kernel = (const void*)rows_kernel<T, NORM, RES, W, 512, 2, true>;
+  if constexpr (W >= 8) {
+    if (l.loop) kernel = (const void*)rows_kernel<T, NORM, RES, W, 0, 4, true>;
+    else if (l.vpt == 1) kernel = (const void*)rows_kernel<T, NORM, RES, W, 0, 1, false>;
+    else if constexpr (W == 16) return launch_rows_shared<T, NORM, RES>(p, l, stream);
+    else kernel = (const void*)rows_kernel<T, NORM, RES, W, 0, 2, false>;
   } else {
-    kernel = l.threads == 32 ? (const void*)rows_kernel<T, NORM, RES, W, 32, 2, false>
-             : l.vpt == 1    ? (const void*)rows_kernel<T, NORM, RES, W, 256, 1, false>
-             : l.threads == 256 ? (const void*)rows_kernel<T, NORM, RES, W, 256, 2, false>
-             : l.threads == 512 ? (const void*)rows_kernel<T, NORM, RES, W, 512, 2, false>
-                                : (const void*)rows_kernel<T, NORM, RES, W, 1024, 2, false>;
+    if (l.loop) kernel = (const void*)rows_kernel<T, NORM, RES, W, 512, 2, true>;
+    else if (l.threads == 32) kernel = l.vpt == 1 ? (const void*)rows_kernel<T, NORM, RES, W, 32, 1, false> : (const void*)rows_kernel<T, NORM, RES, W, 32, 2, false>;
+    else if (l.threads == 256) kernel = l.vpt == 1 ? (const void*)rows_kernel<T, NORM, RES, W, 256, 1, false> : (const void*)rows_kernel<T, NORM, RES, W, 256, 2, false>;
+    else kernel = l.threads == 512 ? (const void*)rows_kernel<T, NORM, RES, W, 512, 2, false> : (const void*)rows_kernel<T, NORM, RES, W, 1024, 2, false>;
   }
   void* args[] = {&p};
   return launch_kernel(kernel, dim3(unsigned(l.grid)), dim3(unsigned(l.threads), unsigned(l.rows)), 0, 0, stream, args);

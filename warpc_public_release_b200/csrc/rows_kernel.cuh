@@ -350,7 +350,7 @@ template <bool NORM>  // 16-byte words of shared memory a thread of these kernel
 constexpr int kRowWords = 2 * (NORM ? 1 : kRowStages);
 
 template <class T, bool NORM, bool RES, int W, int NT, int VPT, bool LOOP>
-__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) rows_kernel(const RowParams p) {
+__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, VPT <= 2 ? 1 : 2) rows_kernel(const RowParams p) {
   static_assert(NORM || !RES, "the residual comes with the norm");
   using S = RowSlot<T, W>;
   using V = typename S::V;
