@@ -226,6 +226,8 @@ WB_DEV void i8_tile_at(const I8Params& p, int tile, int& tm, int& tn) {
   tm = first + in % rows, tn = in / rows;
 }
 
+WB_DEV void i8_prefetch(const float* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // 32 channels' scales (and biases), from memory every lane reads alike
 WB_DEV void i8_channel(const float* src, int n, int N, float* out) {
   if (n + 32 <= N) {
@@ -244,37 +246,42 @@ WB_DEV void i8_channel(const float* src, int n, int N, float* out) {
 // neighbouring memory, as many rows at a time as that leaves lanes for.
 template <class T, int U>
 WB_DEV void i8_store_rows(uint32_t copy, T* out, int m0, int M, int n0, int N, long long ldc, uint32_t lane) {
-  constexpr int LANES = 128 / U < 32 ? 128 / U : 32, ROWS = 32 / LANES, E = U / int(sizeof(T));
-#pragma unroll 4
-  for (uint32_t i = 0; i < 32; i += ROWS) {
-    const uint32_t row = i + lane / LANES;
+  constexpr int LANES = 128 / U < 32 ? 128 / U : 32, ROWS = 32 / LANES, E = U / int(sizeof(T)), AT_ONCE = 8;
+  const uint32_t mine = lane / LANES;
 #pragma unroll
-    for (uint32_t byte = (lane % LANES) * U; byte < 128; byte += LANES * U) {
-      const uint32_t at = copy + row * 128u + (((byte >> 4) ^ (row & 7u)) << 4) + (byte & 15u);
-      const int n = n0 + int(byte) / int(sizeof(T));
-      if (m0 + int(row) >= M || n >= N) continue;
-      T* const to = out + (long long)(m0 + int(row)) * ldc + n;
-      T v[E];
-      if constexpr (U == 8) {
-        uint2 w;
-        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(at) : "memory");
-        memcpy(v, &w, 8);
-        if (n + E <= N) *reinterpret_cast<uint2*>(to) = w;
-      } else if constexpr (U == 4) {
-        uint32_t w;
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
-        memcpy(v, &w, 4);
-        if (n + E <= N) *reinterpret_cast<uint32_t*>(to) = w;
-      } else {
-        uint16_t w;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at) : "memory");
-        memcpy(v, &w, 2);
-        *reinterpret_cast<uint16_t*>(to) = w;
+  for (uint32_t byte = (lane % LANES) * U, pass = 0; pass < 128 / (LANES * U); ++pass, byte += LANES * U) {
+    const int n = n0 + int(byte) / int(sizeof(T));
+#pragma unroll 1
+    for (uint32_t i = 0; i < 32; i += ROWS * AT_ONCE) {
+      uint2 w[AT_ONCE];
+#pragma unroll
+      for (uint32_t j = 0; j < AT_ONCE; ++j) {
+        const uint32_t row = i + j * ROWS + mine, at = copy + row * 128u + (((byte >> 4) ^ (row & 7u)) << 4) + (byte & 15u);
+        if constexpr (U == 8) {
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[j].x), "=r"(w[j].y) : "r"(at) : "memory");
+        } else if constexpr (U == 4) {
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[j].x) : "r"(at) : "memory");
+        } else {
+          uint16_t d;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(d) : "r"(at) : "memory");
+          w[j].x = d;
+        }
       }
-      if (E > 1 && n + E > N) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (n + e < N) to[e] = v[e];
+      for (uint32_t j = 0; j < AT_ONCE; ++j) {
+        const int m = m0 + int(i + j * ROWS + mine);
+        T* const to = out + (long long)m * ldc + n;
+        if (m < M && n + E <= N) {
+          if constexpr (U == 8) *reinterpret_cast<uint2*>(to) = w[j];
+          else if constexpr (U == 4) *reinterpret_cast<uint32_t*>(to) = w[j].x;
+          else *reinterpret_cast<uint16_t*>(to) = uint16_t(w[j].x);
+        } else if (E > 1 && m < M) {  // the row ends inside
+          T v[E];
+          memcpy(v, &w[j], U);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (n + e < N) to[e] = v[e];
+        }
       }
     }
   }
@@ -362,6 +369,10 @@ __global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(con
       i8_tile_at(p, tile, tm, tn);
       const int m0 = (tm * C::CG + int(rank)) * 128 + int(q) * 32, n0 = tn * C::NT + int(side) * 32 * BLOCKS;
       const float sa = m0 + int(lane) < p.M ? __ldg(p.sa + m0 + lane) : 0.0f;
+      if (int(lane) < BLOCKS && n0 + 32 * int(lane) < p.N) {  // a block's scales are a line
+        i8_prefetch(p.sb + n0 + 32 * int(lane));
+        if (p.bias != nullptr) i8_prefetch(p.bias + n0 + 32 * int(lane));
+      }
       if (!i8_wait_warp(p, abort_addr, ctrl + offsetof(I8Ctrl, acc_full) + 8 * acc, acc_phase, I8_WAIT_ACC_FULL, acc)) break;
       tc_fence_after();
       const uint32_t from = tmem + acc * C::NT + side * 32u * BLOCKS + (q << 21);
@@ -513,13 +524,21 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
     __syncwarp();
   }
   cluster_wait();
+  // what the end needs from memory, while the MMAs run: this lane's four channels, and the tokens this CTA finishes (one a lane)
+  const int n = n0 + 4 * int(lane), m_first = m0 + int(rank) * slice;
+  float sb[4], add[4], sa[C::NT / 32];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sb[i] = n + i < p.N ? __ldg(p.sb + n + i) : 0.0f, add[i] = p.bias != nullptr && n + i < p.N ? __ldg(p.bias + n + i) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < C::NT / 32; ++i) sa[i] = m_first + 32 * i + int(lane) < p.M ? __ldg(p.sa + m_first + 32 * i + lane) : 0.0f;
   if (warp >= 4 && i8_wait_warp(p, abort_addr, ctrl + offsetof(I8Ctrl, acc_full), 0, I8_WAIT_ACC_FULL, 0)) {
     tc_fence_after();
     const uint32_t q = warp & 3u;
     const int here = min(C::NT, p.M - m0);
-    const uint32_t word = (q * 32u + lane) * 4u;
-    int dest = 0, local = 0;
-    uint32_t to = mapa(parts, 0);
+    // this warp's channels of token 0 of the slot that this CTA has in the first CTA of the cluster
+    const uint32_t word = rank * uint32_t(slice) * 512u + (q * 32u + lane) * 4u;
+    uint32_t dest = 0, to = mapa(parts, 0) + word;
+    int left = slice;
 #pragma unroll 1
     for (int b = 0; 32 * b < here; ++b) {
       uint32_t v[32];
@@ -528,8 +547,9 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         if (32 * b + i < here) {
-          st_cluster_u32(to + (rank * uint32_t(slice) + uint32_t(local)) * 512u + word, v[i]);
-          if (++local == slice) local = 0, ++dest, to = mapa(parts, min(uint32_t(dest), split - 1u));
+          st_cluster_u32(to, v[i]);
+          to += 512u;
+          if (--left == 0) left = slice, dest = min(dest + 1u, split - 1u), to = mapa(parts, dest) + word;
         }
       }
     }
@@ -540,31 +560,31 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
   cluster_wait();
   if (i8_ld_abort(abort_addr) == 0u) {
     T* const out = static_cast<T*>(p.C);
-    const int n = n0 + 4 * int(lane);
-    float sb[4], add[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sb[i] = n + i < p.N ? __ldg(p.sb + n + i) : 0.0f, add[i] = p.bias != nullptr && n + i < p.N ? __ldg(p.bias + n + i) : 0.0f;
-    for (int i = int(warp); i < slice; i += 8) {
-      const int m = m0 + int(rank) * slice + i;
-      if (int(rank) * slice + i >= C::NT || m >= p.M) break;
-      int sum[4] = {0, 0, 0, 0};
-      for (uint32_t s = 0; s < split; ++s) {
-        int a, b, c, d;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(parts + (s * uint32_t(slice) + uint32_t(i)) * 512u + lane * 16u) : "memory");
-        sum[0] += a, sum[1] += b, sum[2] += c, sum[3] += d;
-      }
-      const float sa = __ldg(p.sa + m);
-      float y[4];
+    for (int r = 0; r < C::NT / 32; ++r) {
+#pragma unroll 2
+      for (int i = 32 * r + int(warp); i < min(slice, 32 * r + 32); i += 8) {
+        const int m = m_first + i;
+        if (int(rank) * slice + i >= C::NT || m >= p.M) break;
+        int sum[4] = {0, 0, 0, 0};
+        for (uint32_t s = 0; s < split; ++s) {
+          int a, b, c, d;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(parts + (s * uint32_t(slice) + uint32_t(i)) * 512u + lane * 16u) : "memory");
+          sum[0] += a, sum[1] += b, sum[2] += c, sum[3] += d;
+        }
+        const float scale = __shfl_sync(0xffffffffu, sa[r], i & 31);
+        float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = p.bias != nullptr ? i8_value(sum[j], sa, sb[j], add[j]) : i8_value(sum[j], sa, sb[j]);
-      T* const to = out + (long long)m * p.ldc + n;
-      if (p.store_bytes >= 4 * int(sizeof(T)) && n + 4 <= p.N) {
-        if constexpr (OUT == I8_FP32) *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
-        else *reinterpret_cast<uint2*>(to) = make_uint2(I8Out<OUT>::two(y[0], y[1]), I8Out<OUT>::two(y[2], y[3]));
-      } else {
+        for (int j = 0; j < 4; ++j) y[j] = p.bias != nullptr ? i8_value(sum[j], scale, sb[j], add[j]) : i8_value(sum[j], scale, sb[j]);
+        T* const to = out + (long long)m * p.ldc + n;
+        if (p.store_bytes >= 4 * int(sizeof(T)) && n + 4 <= p.N) {
+          if constexpr (OUT == I8_FP32) *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+          else *reinterpret_cast<uint2*>(to) = make_uint2(I8Out<OUT>::two(y[0], y[1]), I8Out<OUT>::two(y[2], y[3]));
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) to[j] = I8Out<OUT>::one(y[j]);
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.N) to[j] = I8Out<OUT>::one(y[j]);
+        }
       }
     }
   }
