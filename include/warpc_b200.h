@@ -246,6 +246,8 @@ typedef struct wg_int8_info {
   int kernel, tile_m, tile_n, split;                        /* what names a program */
   int tiles, grid, cluster, threads, dynsmem, depth;        /* its launch */
 } wg_int8_info;
+/* The program the rule picks for M tokens, N channels, depth K (where the output's rows are 16-byte aligned; rows that are not cost
+ * some programs more, and a launch takes that into account). */
 int wg_int8_choose(int M, int N, int K, wg_int8_info* out);
 
 /* A plan for one weight matrix: dBt is N x K signed 8-bit (a row a channel), 16-byte aligned, ldb a multiple of 16; dScaleB

@@ -205,14 +205,16 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
   return WG_E_VARIANT;
 }
 
-// Which program, by estimated microseconds: what a launch costs besides its k-steps, plus its k-steps, measured on B200.
-//   gemv   2 us, and 0.21 / 0.28 / 0.45 / 0.77 us a megabyte of weights for 1 / 2 / 4 / 8 tokens (4096 x 4096: 5.5 / 6.6 / 9.4 / 14.8)
-//   few    4.9 us + 0.195 a k-step with 32 tokens, 6.4 + 0.24 with 64 (4096 x 4096: 32 k-steps 11.3, shared by two CTAs 8.0, by four
-//          6.8), 0.3 more where a cluster shares K; the weights out of memory rather than the L2 add 0.11 us a megabyte
-//   tile   per tile the slower of its k-steps and its store, the launch once (4096^3: 0.35 us a k-step with 256 x 256, 0.24 with
-//          256 x 128, 0.27 with 128 x 128, 0.21 with 128 x 64; 4096 x 4096 x 1024: a tile every 3.1, 2.3, 2.8, 2.1)
+// Which program, by estimated microseconds: what a launch costs besides its k-steps, plus its k-steps, as measured on a B200 with
+// launches back to back.
+//   gemv   1.7 us, and 0.2 / 0.3 / 0.5 / 0.9 us a megabyte of weights for 1 / 2 / 4 / 8 tokens (2048 x 2048: 2.9 / 3.2 / 4.0 / 6.1)
+//   few    512 channels, 32 tokens: 3.7 us with one k-step, 9.9 with 32, 5.2 with 32 shared by four CTAs; 64 tokens: 4.9, 11.4, 5.9;
+//          weights out of memory rather than the L2 add 0.11 us a megabyte
+//   tile   256 x 512 with one k-step / 32: 128 x 64 3.5 / 10.4, 128 x 128 3.9 / 13.5, 256 x 128 3.9 / 11.2, 256 x 256 4.9 / 14.3 (more
+//          a k-step with every SM at work); of several tiles each takes the slower of its k-steps and its store (4096 x 4096 x 1024);
+//          rows of Y that the copy engine cannot write: 0.7, 0.8, 0.8, 2.2 a tile
 // Clusters that run at once (a GPC holds a whole number of them): 74 of two CTAs, 32 of four, 16 of eight.
-int i8_choose(int M, int N, int K, wg_int8_info* o) {
+int i8_choose(int M, int N, int K, bool aligned, wg_int8_info* o) {
   std::memset(o, 0, sizeof *o);
   const int kt = (K + 127) / 128;
   auto up = [](long long a, long long b) { return (a + b - 1) / b; };
@@ -223,22 +225,23 @@ int i8_choose(int M, int N, int K, wg_int8_info* o) {
   };
   if (M <= 8) {
     const int t = M <= 1 ? 0 : M <= 2 ? 1 : M <= 4 ? 2 : 3;
-    static const double mb[] = {0.21, 0.28, 0.45, 0.77};
+    static const double mb[] = {0.2, 0.3, 0.5, 0.9};
     // four channels a warp: warps enough to keep the loads of a whole machine in flight, each with 512 values of K at least
     int wk = 1;
     while (wk < 8 && up(N, 4) * wk < (M <= 1 ? 4096 : 2048) && K > 512 * wk) wk *= 2;
-    take(1.9 + megabytes * mb[t], WG_INT8_GEMV, 1 << t, 0, wk);
+    take(1.7 + megabytes * mb[t], WG_INT8_GEMV, 1 << t, 0, wk);
   }
   for (int t = 32; t <= 64; t *= 2)
     for (int s = 1; s <= 8 && s <= kt; s *= 2) {
       static const int at_once[] = {0, 148, 74, 0, 32, 0, 0, 0, 16};
-      const double waves = double(up(up(M, t) * up(N, 128), at_once[s]));
-      take(waves * ((t == 32 ? 4.9 : 6.4) + (t == 32 ? 0.195 : 0.24) * double(up(kt, s))) + (s > 1 ? 0.3 : 0.0) + 0.11 * megabytes, WG_INT8_FEW, t, 128, s);
+      const double waves = double(up(up(M, t) * up(N, 128), at_once[s])), steps = double(up(kt, s));
+      take(waves * (t == 32 ? 3.2 + 0.3 / s + 0.2 * steps : 3.6 + 1.1 / s + 0.22 * steps) + 0.11 * megabytes, WG_INT8_FEW, t, 128, s);
     }
-  static const struct { int m, n; double launch, step, store; } tiles[] = {{256, 256, 5.8, 0.35, 3.1}, {256, 128, 4.8, 0.237, 2.3}, {128, 128, 4.6, 0.274, 2.8}, {128, 64, 4.2, 0.209, 2.1}};
+  static const struct { int m, n; double launch, step, store, scattered; } tiles[] = {
+      {256, 256, 4.7, 0.35, 3.1, 2.2}, {256, 128, 3.7, 0.235, 2.3, 0.8}, {128, 128, 3.6, 0.29, 2.8, 0.8}, {128, 64, 3.2, 0.21, 2.1, 0.7}};
   for (const auto& t : tiles) {
-    const double each = double(up(up(M, t.m) * up(N, t.n), kSms / (t.m / 128)));
-    take(t.launch + t.step * kt + (each - 1) * std::max(t.step * kt, t.store) + 0.11 * megabytes, WG_INT8_TILE, t.m, t.n, 1);
+    const double each = double(up(up(M, t.m) * up(N, t.n), kSms / (t.m / 128))), store = t.store + (aligned ? 0.0 : t.scattered);
+    take(t.launch + t.step * kt + (each - 1) * std::max(t.step * kt, store) + (aligned ? 0.0 : t.scattered) + 0.11 * megabytes, WG_INT8_TILE, t.m, t.n, 1);
   }
   return i8_derive(M, N, K, o);
 }
@@ -317,7 +320,7 @@ extern "C" int wg_norm_quantise_rows(int device, int M, int K, int dtype, const 
 extern "C" int wg_int8_choose(int M, int N, int K, wg_int8_info* out) {
   if (!out || M <= 0 || N <= 0 || K <= 0) return WG_E_ARG;
   if (K > kMaxK || M > kMaxSize || N > kMaxSize) return WG_E_LIMIT;
-  return i8_choose(M, N, K, out);
+  return i8_choose(M, N, K, true, out);
 }
 
 extern "C" int wg_int8_plan_create(int device, int N, int K, const signed char* dBt, long long ldb, const float* dScaleB, const float* dBias, int out_dtype,
@@ -376,8 +379,10 @@ extern "C" int wg_int8_launch(void* plan, int M, const signed char* dA, long lon
   if (M > kMaxSize) return WG_E_LIMIT;
   if (M == 0) return WG_OK;
   if (!dA || !dScaleA || !dC || !aligned(dA, 16) || !aligned(dScaleA, 4) || !aligned(dC, unsigned(size))) return WG_E_ARG;
+  int store_bytes = 16;  // what the rows of C are aligned to
+  while (store_bytes > size && !(aligned(dC, unsigned(store_bytes)) && (ldc * size) % store_bytes == 0)) store_bytes /= 2;
   wg_int8_info li = pl->named;
-  int r = li.kernel ? i8_derive(M, pl->N, pl->K, &li) : i8_choose(M, pl->N, pl->K, &li);
+  int r = li.kernel ? i8_derive(M, pl->N, pl->K, &li) : i8_choose(M, pl->N, pl->K, store_bytes == 16, &li);
   if (r != WG_OK) return r;
   I8Params p;
   std::memset(&p, 0, sizeof p);
@@ -386,7 +391,7 @@ extern "C" int wg_int8_launch(void* plan, int M, const signed char* dA, long lon
   p.depth = li.depth, p.group = 8, p.wk = li.split;
   p.A = reinterpret_cast<const int8_t*>(dA), p.Bt = pl->Bt, p.lda = lda, p.ldb = pl->ldb, p.ldc = ldc;
   p.sa = dScaleA, p.sb = pl->sb, p.bias = pl->bias, p.C = dC, p.status = pl->d_status, p.timeout_ns = pl->timeout_ns;
-  for (p.store_bytes = 16; p.store_bytes > size && !(aligned(dC, unsigned(p.store_bytes)) && (ldc * size) % p.store_bytes == 0);) p.store_bytes /= 2;
+  p.store_bytes = store_bytes;
   WG_ON_DEVICE(pl->device);
   CUtensorMap map_a, map_c;
   std::memset(&map_a, 0, sizeof map_a), std::memset(&map_c, 0, sizeof map_c);

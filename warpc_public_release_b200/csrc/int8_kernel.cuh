@@ -531,22 +531,25 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
   for (int i = 0; i < 4; ++i) sb[i] = n + i < p.N ? __ldg(p.sb + n + i) : 0.0f, add[i] = p.bias != nullptr && n + i < p.N ? __ldg(p.bias + n + i) : 0.0f;
 #pragma unroll
   for (int i = 0; i < C::NT / 32; ++i) sa[i] = m_first + 32 * i + int(lane) < p.M ? __ldg(p.sa + m_first + 32 * i + lane) : 0.0f;
-  if (warp >= 4 && i8_wait_warp(p, abort_addr, ctrl + offsetof(I8Ctrl, acc_full), 0, I8_WAIT_ACC_FULL, 0)) {
+  if (i8_wait_warp(p, abort_addr, ctrl + offsetof(I8Ctrl, acc_full), 0, I8_WAIT_ACC_FULL, 0)) {
     tc_fence_after();
-    const uint32_t q = warp & 3u;
-    const int here = min(C::NT, p.M - m0);
-    // this warp's channels of token 0 of the slot that this CTA has in the first CTA of the cluster
+    // all eight warps, two a quarter of the lanes, half the tokens each (warps 0-3 are done with their roles)
+    constexpr int HALF = C::NT / 2;
+    if (warp < 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(ctrl + uint32_t(offsetof(I8Ctrl, tmem_base))) : "memory");
+    const uint32_t q = warp & 3u, t0 = warp < 4 ? HALF : 0;
+    const int here = min(HALF, p.M - m0 - int(t0));
+    // this warp's channels, in the slot that this CTA has in the CTA of the cluster that finishes the token
     const uint32_t word = rank * uint32_t(slice) * 512u + (q * 32u + lane) * 4u;
-    uint32_t dest = 0, to = mapa(parts, 0) + word;
-    int left = slice;
-#pragma unroll 1
-    for (int b = 0; 32 * b < here; ++b) {
-      uint32_t v[32];
-      tmem_ld_x32(tmem + (q << 21) + 32 * b, v);
+    uint32_t dest = t0 / uint32_t(slice);
+    int left = slice - int(t0 % uint32_t(slice));
+    uint32_t to = mapa(parts, min(dest, split - 1u)) + word + uint32_t(slice - left) * 512u;
+    if (here > 0) {
+      uint32_t v[HALF];
+      tmem_ld<HALF>(tmem + (q << 21) + t0, v);
       tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (32 * b + i < here) {
+      for (int i = 0; i < HALF; ++i) {
+        if (i < here) {
           st_cluster_u32(to, v[i]);
           to += 512u;
           if (--left == 0) left = slice, dest = min(dest + 1u, split - 1u), to = mapa(parts, dest) + word;
