@@ -257,7 +257,8 @@ int wg_int8_plan_create(int device, int N, int K, const signed char* dBt, long l
 /* C[m, n] = dScaleA[m] * dScaleB[n] * sum_k A[m, k] * Bt[n, k] (+ dBias[n]) for M tokens, on `cuda_stream`: the sum in 32-bit
  * integers (exact; the same bits every launch, whatever the program), scaled in fp32, rounded once to the output type.  dA is M x K signed
  * 8-bit, 16-byte aligned, lda a multiple of 16; ldc >= N, any alignment of dC (16-byte aligned rows are the fast ones).
- * A row's last 16-byte piece is read whole; what it holds past K does not matter.  M = 0 is no work.  Launches of one plan on
+ * A row's last 16-byte piece is read whole; what it holds past K does not matter.  Rows of A and Bt that start on 128-byte boundaries
+ * are the fast ones (a stride that is no multiple of 32 bytes costs up to a third).  M = 0 is no work.  Launches of one plan on
  * several streams at once are fine. */
 int wg_int8_launch(void* plan, int M, const signed char* dA, long long lda, const float* dScaleA, void* dC, long long ldc, void* cuda_stream);
 /* Name the program of the launches that follow (kernel, tile_m, tile_n, split; the rest is derived), NULL: the rule's again.

@@ -135,7 +135,8 @@ struct I8Plan {
   const int8_t* Bt = nullptr;
   long long ldb = 0;
   const float *sb = nullptr, *bias = nullptr;
-  CUtensorMap map_b128, map_b64;  // the weights in boxes of 128 and of 64 rows
+  CUtensorMap map_b128, map_b64;            // the weights in boxes of 128 and of 64 rows
+  CUtensorMap map_b128_last, map_b64_last;  // and their last rows, fewer than that, in one box
   uint32_t* d_status = nullptr;
   unsigned long long timeout_ns = 2000ull * 1000ull * 1000ull;
   wg_int8_info named{};  // the program a caller named, or kernel 0
@@ -147,6 +148,10 @@ int encode_rows(CUtensorMap* map, CUtensorMapDataType type, int size, const void
   cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
   cuuint64_t strides[1] = {cuuint64_t(ld) * cuuint64_t(size)};
   cuuint32_t box[2] = {cuuint32_t(128 / size), cuuint32_t(box_rows)}, estr[2] = {1, 1};
+  if (box_rows == 0) {  // no such rows: a map that nothing loads through
+    std::memset(map, 0, sizeof *map);
+    return WG_OK;
+  }
   const CUresult r = enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? WG_OK : int(r);
@@ -213,7 +218,7 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
 //   tile   256 x 512 with one k-step / 32: 128 x 64 3.5 / 10.4, 128 x 128 3.9 / 13.5, 256 x 128 3.9 / 11.2, 256 x 256 4.9 / 14.3 (more
 //          a k-step with every SM at work); of several tiles each takes the slower of its k-steps and its store (4096 x 4096 x 1024);
 //          rows of Y that the copy engine cannot write: 0.7, 0.8, 0.8, 2.2 a tile
-// Clusters that run at once (a GPC holds a whole number of them): 74 of two CTAs, 32 of four, 16 of eight.
+// Clusters that run at once (a GPC holds a whole number of them): 74 of two CTAs, 33 of four, 15 of eight.
 int i8_choose(int M, int N, int K, bool aligned, wg_int8_info* o) {
   std::memset(o, 0, sizeof *o);
   const int kt = (K + 127) / 128;
@@ -233,7 +238,7 @@ int i8_choose(int M, int N, int K, bool aligned, wg_int8_info* o) {
   }
   for (int t = 32; t <= 64; t *= 2)
     for (int s = 1; s <= 8 && s <= kt; s *= 2) {
-      static const int at_once[] = {0, 148, 74, 0, 32, 0, 0, 0, 16};
+      static const int at_once[] = {0, 148, 74, 0, 33, 0, 0, 0, 15};
       const double waves = double(up(up(M, t) * up(N, 128), at_once[s])), steps = double(up(kt, s));
       take(waves * (t == 32 ? 3.2 + 0.3 / s + 0.2 * steps : 3.6 + 1.1 / s + 0.22 * steps) + 0.11 * megabytes, WG_INT8_FEW, t, 128, s);
     }
@@ -260,7 +265,7 @@ struct I8Kernels {
     for (const void* fn : fns) WG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kI8MaxSmem)));
     return WG_OK;
   }
-  static int run(const wg_int8_info& li, cudaStream_t stream, CUtensorMap* a, CUtensorMap* b, CUtensorMap* c, I8Params* p) {
+  static int run(const wg_int8_info& li, cudaStream_t stream, CUtensorMap* a, CUtensorMap* a_last, CUtensorMap* b, CUtensorMap* b_last, CUtensorMap* c, I8Params* p) {
     if (li.kernel == WG_INT8_GEMV) {
       void* args[] = {p};
       switch (li.tile_m) {
@@ -271,10 +276,10 @@ struct I8Kernels {
       }
     }
     if (li.kernel == WG_INT8_FEW) {
-      void* args[] = {a, b, p};
+      void* args[] = {a, a_last, b, b_last, p};
       return li.tile_m == 32 ? launch((const void*)i8_few_kernel<FewCfg<32>, OUT>, li, stream, args) : launch((const void*)i8_few_kernel<FewCfg<64>, OUT>, li, stream, args);
     }
-    void* args[] = {a, b, c, p};
+    void* args[] = {a, a_last, b, b_last, c, p};
     if (li.tile_m == 256) return li.tile_n == 256 ? launch((const void*)i8_tile_kernel<TileCfg<256, 256>, OUT>, li, stream, args) : launch((const void*)i8_tile_kernel<TileCfg<256, 128>, OUT>, li, stream, args);
     return li.tile_n == 128 ? launch((const void*)i8_tile_kernel<TileCfg<128, 128>, OUT>, li, stream, args) : launch((const void*)i8_tile_kernel<TileCfg<128, 64>, OUT>, li, stream, args);
   }
@@ -337,6 +342,8 @@ extern "C" int wg_int8_plan_create(int device, int N, int K, const signed char* 
   pl->Bt = reinterpret_cast<const int8_t*>(dBt), pl->ldb = ldb, pl->sb = dScaleB, pl->bias = dBias;
   int r = encode_rows(&pl->map_b128, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dBt, N, K, ldb, 128);
   if (r == WG_OK) r = encode_rows(&pl->map_b64, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dBt, N, K, ldb, 64);
+  if (r == WG_OK) r = encode_rows(&pl->map_b128_last, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dBt, N, K, ldb, N % 128);
+  if (r == WG_OK) r = encode_rows(&pl->map_b64_last, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dBt, N, K, ldb, N % 64);
   if (r == WG_OK) r = int(cudaMalloc(&pl->d_status, 4 * sizeof(uint32_t)));
   if (r == WG_OK) r = int(cudaMemsetAsync(pl->d_status, 0, 4 * sizeof(uint32_t), 0));
   if (r == WG_OK) r = int(cudaStreamSynchronize(0));  // zero before any stream, blocking or not, can launch on the plan
@@ -393,20 +400,24 @@ extern "C" int wg_int8_launch(void* plan, int M, const signed char* dA, long lon
   p.sa = dScaleA, p.sb = pl->sb, p.bias = pl->bias, p.C = dC, p.status = pl->d_status, p.timeout_ns = pl->timeout_ns;
   p.store_bytes = store_bytes;
   WG_ON_DEVICE(pl->device);
-  CUtensorMap map_a, map_c;
-  std::memset(&map_a, 0, sizeof map_a), std::memset(&map_c, 0, sizeof map_c);
-  CUtensorMap* map_b = li.kernel == WG_INT8_TILE && li.tile_n / li.cluster == 64 ? &pl->map_b64 : &pl->map_b128;
-  if (li.kernel != WG_INT8_GEMV)
-    if ((r = encode_rows(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dA, M, pl->K, lda, li.kernel == WG_INT8_FEW ? li.tile_m : 128)) != WG_OK) return r;
+  CUtensorMap map_a, map_a_last, map_c;
+  std::memset(&map_a, 0, sizeof map_a), std::memset(&map_a_last, 0, sizeof map_a_last), std::memset(&map_c, 0, sizeof map_c);
+  const bool b64 = li.kernel == WG_INT8_TILE && li.tile_n / li.cluster == 64;
+  CUtensorMap *map_b = b64 ? &pl->map_b64 : &pl->map_b128, *map_b_last = b64 ? &pl->map_b64_last : &pl->map_b128_last;
+  if (li.kernel != WG_INT8_GEMV) {
+    const int box = li.kernel == WG_INT8_FEW ? li.tile_m : 128;
+    if (M >= box && (r = encode_rows(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dA, M, pl->K, lda, box)) != WG_OK) return r;
+    if ((r = encode_rows(&map_a_last, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dA, M, pl->K, lda, M % box)) != WG_OK) return r;
+  }
   if (li.kernel == WG_INT8_TILE && p.store_bytes == 16) {
     const CUtensorMapDataType type = pl->out == WG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : pl->out == WG_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     if ((r = encode_rows(&map_c, type, size, dC, M, pl->N, ldc, 32)) != WG_OK) return r;
   }
   const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   switch (pl->out) {
-    case WG_BF16: return I8Kernels<I8_BF16>::run(li, stream, &map_a, map_b, &map_c, &p);
-    case WG_FP16: return I8Kernels<I8_FP16>::run(li, stream, &map_a, map_b, &map_c, &p);
-    default: return I8Kernels<I8_FP32>::run(li, stream, &map_a, map_b, &map_c, &p);
+    case WG_BF16: return I8Kernels<I8_BF16>::run(li, stream, &map_a, &map_a_last, map_b, map_b_last, &map_c, &p);
+    case WG_FP16: return I8Kernels<I8_FP16>::run(li, stream, &map_a, &map_a_last, map_b, map_b_last, &map_c, &p);
+    default: return I8Kernels<I8_FP32>::run(li, stream, &map_a, &map_a_last, map_b, map_b_last, &map_c, &p);
   }
 }
 

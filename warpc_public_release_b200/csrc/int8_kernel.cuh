@@ -114,10 +114,26 @@ struct I8Cfg {
   static_assert(NT % 32 == 0 && NT <= 256 && Q_BYTES % 1024 == 0, "tile");
 };
 
-// Producer, one lane: k-steps [kb, ke) of a tile, two boxes a step.  For a pair both CTAs' bytes arrive on the leader's barrier.
+// The rows that one CTA loads of an operand for a tile: its block of `box` rows, through the operand's map of whole boxes or, for the
+// last rows, through one whose box is as high as they are.  A box is never asked for rows past the operand's end: those are
+// zeros for the asking but not for free (48 x 5888 x 896 in 128-row boxes, 10.4 us, in 48-row ones 5.9; 16 x 5888 x 896 12.3 and 5.7: every CTA's missing rows
+// are fetched from one place).  The slot's other rows hold whatever was there; nobody looks at what they are multiplied to.
+struct I8Rows {
+  bool last;   // through the map of the last rows
+  int row, rows;
+};
+WB_DEV I8Rows i8_rows(int block, int size, int box) {
+  const int whole = size / box, rest = size % box;
+  if (block < whole) return {false, block * box, box};
+  if (rest != 0 && (block == whole || whole == 0)) return {true, whole * box, rest};
+  return {false, 0, box};  // no rows left for this CTA of a pair: any will do
+}
+
+// Producer, one lane: k-steps [kb, ke) of a tile, two boxes a step.  For a pair both CTAs' bytes (`rows` of them, 128 each) arrive
+// on the leader's barrier.
 template <class C>
 WB_DEV bool i8_load(const I8Params& p, uint32_t abort_addr, uint32_t ring, uint32_t ctrl, uint32_t rank, const void* map_p, int row_p, const void* map_q,
-                    int row_q, int kb, int ke, uint32_t& stage, uint32_t& phase) {
+                    int row_q, int rows, int kb, int ke, uint32_t& stage, uint32_t& phase) {
   const uint32_t full0 = ctrl + offsetof(I8Ctrl, full), empty0 = ctrl + offsetof(I8Ctrl, empty);
   const uint32_t full_to = C::CG == 2 ? mapa(full0, 0) : full0;
   const uint64_t policy = l2_policy_evict_normal();
@@ -126,11 +142,11 @@ WB_DEV bool i8_load(const I8Params& p, uint32_t abort_addr, uint32_t ring, uint3
   while (left != 0u) {
     uint32_t gave_up;
     if constexpr (C::KSUB == 1)
-      gave_up = load_k_loop<C::CG, 128>(1u, left, uint32_t(p.depth), stage, phase, x, empty0, full0, full_to, rank == 0 ? 1u : 0u, uint32_t(C::CG * C::STAGE),
+      gave_up = load_k_loop<C::CG, 128>(1u, left, uint32_t(p.depth), stage, phase, x, empty0, full0, full_to, rank == 0 ? 1u : 0u, uint32_t(rows * 128),
                                         ring, uint32_t(C::STAGE), uint32_t(C::P_BYTES), map_p, row_p, map_q, row_q, 1u << 14, 0u, policy);
     else
       gave_up = load_rounds<C::CG, C::KSUB, 128>(1u, left, uint32_t(p.depth), stage, phase, x, empty0, full0, full_to, rank == 0 ? 1u : 0u,
-                                                 uint32_t(C::CG * C::STAGE), ring, uint32_t(C::ROUND), uint32_t(C::P_BYTES), map_p, row_p, map_q, row_q,
+                                                 uint32_t(rows * 128), ring, uint32_t(C::ROUND), uint32_t(C::P_BYTES), map_p, row_p, map_q, row_q,
                                                  1u << 14, 0u, uint32_t(C::STAGE), policy);
     if (gave_up != 0u && !i8_wait_lane(p, abort_addr, empty0 + 8 * stage, phase ^ 1u, I8_WAIT_EMPTY, stage)) return false;
   }
@@ -288,7 +304,8 @@ WB_DEV void i8_store_rows(uint32_t copy, T* out, int m0, int M, int n0, int N, l
 }
 
 template <class C, int OUT>
-__global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+__global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_last,
+                                                         const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_last,
                                                          const __grid_constant__ CUtensorMap map_c, const __grid_constant__ I8Params p) {
   using L = I8Tile<C, OUT>;
   using T = typename I8Out<OUT>::T;
@@ -311,7 +328,10 @@ __global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(con
     fence_mbar_init();
     __threadfence_block();  // the abort word too, ahead of the relaxed arrival
   }
-  if (warp == 2 && lane == 0) prefetch_tmap(&map_a), prefetch_tmap(&map_b), prefetch_tmap(&map_c);
+  if (warp == 2 && lane == 0) {
+    prefetch_tmap(p.M >= 128 ? &map_a : &map_a_last), prefetch_tmap(&map_b);
+    if (p.store_bytes == 16) prefetch_tmap(&map_c);
+  }
   __syncwarp();
   if constexpr (C::CG == 2) cluster_arrive_relaxed(), cluster_wait();
   else __syncthreads();
@@ -335,7 +355,10 @@ __global__ void __launch_bounds__(I8Tile<C, OUT>::THREADS, 1) i8_tile_kernel(con
       for (int tile = first; ok && tile < ntiles; tile += step) {
         int tm, tn;
         i8_tile_at(p, tile, tm, tn);
-        ok = i8_load<C>(p, abort_addr, ring, ctrl, rank, &map_a, (tm * C::CG + int(rank)) * 128, &map_b, tn * C::NT + int(rank) * C::Q_ROWS, 0, p.kt, stage, phase);
+        const I8Rows a = i8_rows(tm * C::CG + int(rank), p.M, 128), b = i8_rows(tn * C::CG + int(rank), p.N, C::Q_ROWS);
+        int rows = a.rows + b.rows;
+        if (C::CG == 2) rows += i8_rows(tm * C::CG + 1 - int(rank), p.M, 128).rows + i8_rows(tn * C::CG + 1 - int(rank), p.N, C::Q_ROWS).rows;
+        ok = i8_load<C>(p, abort_addr, ring, ctrl, rank, a.last ? &map_a_last : &map_a, a.row, b.last ? &map_b_last : &map_b, b.row, rows, 0, p.kt, stage, phase);
       }
       if (ok) i8_load_done(p, abort_addr, ctrl, stage, phase);
     }
@@ -471,7 +494,8 @@ struct I8Few {
 };
 
 template <class C, int OUT>
-__global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+__global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_last,
+                                                     const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_last,
                                                      const __grid_constant__ I8Params p) {
   static_assert(C::CG == 1, "one CTA a tile");
   using L = I8Few<C>;
@@ -495,7 +519,7 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
     asm volatile("st.shared.u32 [%0], 0;" ::"r"(abort_addr) : "memory");
     fence_mbar_init();
   }
-  if (warp == 2 && lane == 0) prefetch_tmap(&map_a), prefetch_tmap(&map_b);
+  if (warp == 2 && lane == 0) prefetch_tmap(p.M >= C::NT ? &map_a : &map_a_last), prefetch_tmap(&map_b);
   __syncthreads();
   cluster_arrive();  // every CTA of the cluster runs before another writes into its shared memory (waited for below)
   if (warp == 1) {   // after the barrier: the first loads go out meanwhile
@@ -513,7 +537,8 @@ __global__ void __launch_bounds__(256) i8_few_kernel(const __grid_constant__ CUt
   if (warp == 0) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0;
-      if (i8_load<C>(p, abort_addr, ring, ctrl, 0u, &map_b, n0, &map_a, m0, kb, ke, stage, phase)) i8_load_done(p, abort_addr, ctrl, stage, phase);
+      const I8Rows a = i8_rows(tm, p.M, C::NT), b = i8_rows(tn, p.N, 128);
+      if (i8_load<C>(p, abort_addr, ring, ctrl, 0u, b.last ? &map_b_last : &map_b, b.row, a.last ? &map_a_last : &map_a, a.row, a.rows + b.rows, kb, ke, stage, phase)) i8_load_done(p, abort_addr, ctrl, stage, phase);
     }
     __syncwarp();
   } else if (warp == 1) {
