@@ -21,7 +21,7 @@
 // What bounds it is memory in the end and instructions on the way: at 6.5 TB/s an SM has about 16 instruction slots a value of a
 // 16-bit row that is only read and quantised.  So the arithmetic is in pairs (f32x2), a 16-bit row's maximum is taken on the packed
 // values, what only the row's scale needs (roots, exact divisions, the sum over the warps) is left to one warp, and a thread
-// holds up to 32 values, so that the reductions are spread over them.
+// holds sixteen values (of 16 bits; eight of 32) and more, so that the reductions are spread over them.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
