@@ -187,6 +187,7 @@ int i8_derive(int M, int N, int K, wg_int8_info* o) {
     if ((o->tile_m != 32 && o->tile_m != 64) || o->tile_n != 128) return WG_E_VARIANT;
     if ((o->split != 1 && o->split != 2 && o->split != 4 && o->split != 8) || o->split > kt) return WG_E_VARIANT;
     const size_t round = kFewKsub * size_t(128 + o->tile_m) * 128, fixed = 1024 + sizeof(I8Ctrl) + size_t(o->split) * up(o->tile_m, o->split) * 512;
+    // (two CTAs an SM, each with half the ring, where there are more tiles than SMs: 32x28672x8192 46.7 -> 49.0 us, 32x40000x4096 42 -> 48)
     o->depth = ring_depth(fixed, round, std::max(2, up(up(kt, o->split), kFewKsub)));
     o->dynsmem = int(fixed + o->depth * round), o->cluster = o->split;
     const long long tiles = (long long)up(M, o->tile_m) * up(N, 128);
